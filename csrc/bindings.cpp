@@ -73,6 +73,18 @@ void kv_page_copy(torch::Tensor src_bases, torch::Tensor dst_bases, torch::Tenso
 void kv_page_slice_copy(torch::Tensor src_bases, torch::Tensor dst_bases, torch::Tensor src_pages,
                         torch::Tensor dst_pages, int64_t src_page_bytes, int64_t dst_page_bytes, int64_t src_off,
                         int64_t dst_off, int64_t nbytes);
+// logits_stats.cu
+void logits_stats(torch::Tensor logits, int64_t V, torch::Tensor ids, int64_t vocab_offset, int64_t K,
+                  torch::Tensor logprobs, torch::Tensor entropy, torch::Tensor lse, torch::Tensor top_vals,
+                  torch::Tensor top_ids);
+// head_stats.cu
+void head_stats(torch::Tensor hidden, torch::Tensor weight, int64_t V, bool tiled, torch::Tensor ids,
+                int64_t vocab_offset, torch::Tensor logprobs, torch::Tensor entropy, torch::Tensor lse,
+                torch::Tensor status);
+// prompt_attention.cu
+void prompt_attention(torch::Tensor out, torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor indptr,
+                      int64_t heads, int64_t kv_heads, int64_t D, int64_t DV, int64_t window, double sm_scale,
+                      c10::optional<torch::Tensor> sinks, torch::Tensor status);
 int64_t nvls_flag_bytes();
 void nvls_allreduce(torch::Tensor out, torch::Tensor x, int64_t uc, int64_t mc, int64_t capacity, int64_t rank,
                     int64_t world, int64_t max_ctas, torch::Tensor status);
@@ -169,6 +181,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("dcp_size") = 1, py::arg("dcp_rank") = 0, py::arg("lse_out") = py::none());
   m.def("kv_page_copy", &kv_page_copy);
   m.def("kv_page_slice_copy", &kv_page_slice_copy);
+  m.def("logits_stats", &logits_stats);
+  m.def("head_stats", &head_stats);
+  m.def("prompt_attention", &prompt_attention);
   m.def("nvls_flag_bytes", &nvls_flag_bytes);
   m.def("nvls_allreduce", &nvls_allreduce);
   m.def("nvls_combine_allreduce", &nvls_combine_allreduce);

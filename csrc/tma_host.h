@@ -4,7 +4,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <cudaTypedefs.h>
-#include <torch/extension.h>
+#include <c10/util/Exception.h>
 
 namespace snb_host {
 

@@ -56,6 +56,10 @@ class _CountingKernels:
             def call(*a, **k):
                 _launches[0] += 2 if (len(a) > 8 and int(a[6]) > 1 and a[7] is not None and a[8]) else 1
                 return fn(*a, **k)
+        elif name == "head_stats":
+            def call(*a, **k):
+                _launches[0] += 2  # the product with its partial statistics, and their join
+                return fn(*a, **k)
         elif name in _HOST_ONLY:
             return fn
         else:

@@ -1,0 +1,84 @@
+"""Causal attention of packed whole prompts: keys and values straight from the projections, no paged cache.
+
+For passes that keep nothing (scoring prompts) and for the first pass of whole prompts. GQA, sliding window and
+learned per-head sinks as in the paged ops (ops/attention.py); the value width may differ from the key width
+(decompressed latent attention: 192 / 128).
+"""
+from typing import Optional
+
+import torch
+
+from .._ext import kernels
+from .attention import _attend_ref
+from .gemm import _status_buf
+
+# (key width, value width) the kernel serves
+HEAD_DIMS = ((64, 64), (128, 128), (192, 128))
+
+
+def prompt_attention_ref(q, k, v, qo_indptr, num_q_heads, num_kv_heads, head_dim, v_head_dim=None, window=0,
+                         sm_scale=None, sinks=None):
+    v_head_dim = head_dim if v_head_dim is None else v_head_dim
+    sm_scale = head_dim ** -0.5 if sm_scale is None else sm_scale
+    T = q.shape[0]
+    out = torch.zeros(T, num_q_heads, v_head_dim, dtype=torch.float32, device=q.device)
+    bounds = qo_indptr.tolist()
+    for a, b in zip(bounds[:-1], bounds[1:]):
+        if b <= a:
+            continue
+        pos = torch.arange(b - a, device=q.device)
+        out[a:b] = _attend_ref(q[a:b].reshape(b - a, num_q_heads, head_dim),
+                               k[a:b].reshape(b - a, num_kv_heads, head_dim).float(),
+                               v[a:b].reshape(b - a, num_kv_heads, v_head_dim).float(), pos, pos, sm_scale, window,
+                               sinks)
+    return out.reshape(T, num_q_heads * v_head_dim)
+
+
+def _rows(x: torch.Tensor) -> torch.Tensor:
+    """x with rows the kernel can read: contiguous, on 16-byte boundaries."""
+    if x.stride(1) != 1 or x.stride(0) % 8 or x.data_ptr() % 16:
+        return x.contiguous()
+    return x
+
+
+def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, qo_indptr: torch.Tensor, num_q_heads: int,
+                     num_kv_heads: int, head_dim: int, v_head_dim: Optional[int] = None, window: int = 0,
+                     sm_scale: Optional[float] = None, sinks: Optional[torch.Tensor] = None,
+                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Tokens [qo_indptr[b], qo_indptr[b + 1]) are prompt b; every token attends to itself and the tokens before it
+    in its prompt (the last `window` of them where window > 0). q [T, num_q_heads * head_dim], k and v [T,
+    num_kv_heads * width]: bf16 or fp16 on CUDA, views with a row stride (columns of a fused projection) included.
+    Returns [T, num_q_heads * v_head_dim]; rows outside every prompt are left as they are."""
+    v_head_dim = head_dim if v_head_dim is None else v_head_dim
+    sm_scale = head_dim ** -0.5 if sm_scale is None else sm_scale
+    if num_kv_heads <= 0 or num_q_heads % num_kv_heads:
+        raise ValueError(f"{num_q_heads} heads do not divide over {num_kv_heads} KV heads")
+    T = q.shape[0]
+    for name, x, width in (("q", q, num_q_heads * head_dim), ("k", k, num_kv_heads * head_dim),
+                           ("v", v, num_kv_heads * v_head_dim)):
+        if tuple(x.shape) != (T, width) or x.dtype != q.dtype:
+            raise ValueError(f"{name} is {tuple(x.shape)} {x.dtype}, expected {(T, width)} {q.dtype}")
+    if qo_indptr.dim() != 1 or qo_indptr.numel() < 1 or qo_indptr.dtype != torch.int32:
+        raise ValueError("qo_indptr must be an int32 vector of prompt bounds")
+    if window < 0 or not sm_scale > 0:
+        raise ValueError(f"window {window} and sm_scale {sm_scale}: a window of 0 (off) or more, a positive scale")
+    if sinks is not None and sinks.numel() != num_q_heads:
+        raise ValueError(f"{sinks.numel()} sinks for {num_q_heads} heads")
+    if out is not None and tuple(out.shape) != (T, num_q_heads * v_head_dim):
+        raise ValueError(f"out is {tuple(out.shape)}, expected {(T, num_q_heads * v_head_dim)}")
+    if not q.is_cuda:
+        r = prompt_attention_ref(q, k, v, qo_indptr, num_q_heads, num_kv_heads, head_dim, v_head_dim, window,
+                                 sm_scale, sinks).to(q.dtype)
+        if out is not None:
+            out.copy_(r)
+            return out
+        return r
+    if q.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"prompt_attention takes bf16 or fp16 on CUDA, got {q.dtype}")
+    if (head_dim, v_head_dim) not in HEAD_DIMS:
+        raise ValueError(f"prompt_attention serves head dims {HEAD_DIMS} on CUDA, got {(head_dim, v_head_dim)}")
+    if out is None:
+        out = torch.empty(T, num_q_heads * v_head_dim, dtype=q.dtype, device=q.device)
+    kernels().prompt_attention(out, _rows(q), _rows(k), _rows(v), qo_indptr, num_q_heads, num_kv_heads, head_dim,
+                               v_head_dim, window, sm_scale, sinks, _status_buf(q.device))
+    return out
