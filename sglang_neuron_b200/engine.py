@@ -163,6 +163,62 @@ class Engine:
             out.append(d)
         return out
 
+    def score(self, prompts: Sequence, top_logprobs_num: int = 0) -> List[Dict]:
+        """How likely the model finds each prompt: the log-probability of every token given the ones before it, the
+        entropy of each of those distributions and, with top_logprobs_num, the best alternatives (temperature 1).
+
+        Prompts (token-id lists or strings) run whole, packed up to max_prefill_tokens tokens a forward, without
+        touching the KV cache or the scheduler. Per prompt: `input_token_logprobs` [[log-probability, id], ...]
+        (None for the first token, which nothing precedes), `input_entropies` and `input_top_logprobs` (also None
+        first). Under tensor parallelism every rank makes the same call."""
+        from .ops.logprobs import MAX_TOP
+        st = get_state()
+        if st.pp_size > 1 or st.attn_dp_size > 1:
+            raise ValueError("score runs on one pipeline stage and one attention group")
+        if not 0 <= top_logprobs_num <= min(MAX_TOP, self.cfg.vocab_size):
+            raise ValueError(f"top_logprobs_num {top_logprobs_num} outside "
+                             f"[0, {min(MAX_TOP, self.cfg.vocab_size)}]")
+        seqs = [self._to_ids(p) for p in prompts]
+        for ids in seqs:
+            if not 0 < len(ids) <= self.args.context_length:
+                raise ValueError(f"a prompt of {len(ids)} tokens; 1 to {self.args.context_length} are served")
+            if min(ids) < 0 or max(ids) >= self.cfg.vocab_size:
+                raise ValueError(f"a token id outside the vocabulary of {self.cfg.vocab_size}")
+        out: List[Dict] = [None] * len(seqs)
+        group: List[int] = []
+        for i in range(len(seqs) + 1):
+            if group and (i == len(seqs) or
+                          sum(len(seqs[j]) for j in group) + len(seqs[i]) > self.args.max_prefill_tokens):
+                self._score_group([seqs[j] for j in group], group, top_logprobs_num, out)
+                group = []
+            if i < len(seqs):
+                if len(seqs[i]) > 1:
+                    group.append(i)
+                else:
+                    out[i] = self._score_result(seqs[i], [], [], [], [], top_logprobs_num)
+        return out
+
+    @staticmethod
+    def _score_result(ids, lp, ent, tl, ti, k: int) -> Dict:
+        d = {"prompt_tokens": len(ids), "input_token_logprobs": [[v, t] for v, t in zip([None] + lp, ids)],
+             "input_entropies": [None] + ent}
+        if k:
+            d["input_top_logprobs"] = [None] + [[[v, t] for v, t in zip(a, b)] for a, b in zip(tl, ti)]
+        return d
+
+    @torch.no_grad()
+    def _score_group(self, seqs, where, k: int, out) -> None:
+        r = self.runner.score_prompts(seqs, k)
+        lp, ent, tl, ti = (t.tolist() for t in (r.logprobs, r.entropy, r.top_logprobs, r.top_ids))
+        if self.runner.cuda:
+            from .ops.gemm import check_status
+            check_status(self.runner.device)  # the reads above have synchronised
+        a = 0
+        for i, ids in zip(where, seqs):
+            b = a + len(ids) - 1
+            out[i] = self._score_result(ids, lp[a:b], ent[a:b], tl[a:b], ti[a:b], k)
+            a = b
+
     def _generate_spec(self, prompts, sps) -> List[Dict]:
         """Speculative (MTP) generation: greedy, host-synchronous verify/accept steps."""
         from .managers.schedule_batch import Req

@@ -41,6 +41,8 @@ class ForwardBatch:
     decode_splits: int = 1
     # speculative decoding: number of query tokens per request in a verify step (1 = plain decode)
     spec_tokens: int = 1
+    # whole prompts, packed by qo_indptr, that neither read nor write the KV pool (scoring)
+    packed_prompts: bool = False
     extra: dict = dataclasses.field(default_factory=dict)
 
     @property

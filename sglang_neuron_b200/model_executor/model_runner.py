@@ -328,6 +328,64 @@ class ModelRunner:
             ("page_upd", torch.int32, 3 * U), ("temperature", torch.float32, B), ("top_p", torch.float32, B),
         ])
 
+    # ------------------------------------------------------------------------------------------
+    # rows whose logits exist at a time when alternatives are asked for (0.8 GB of bf16 logits at 201088 tokens)
+    SCORE_ROWS = 2048
+
+    def score_prompts(self, prompts: List[List[int]], top_k: int = 0):
+        """One forward over whole prompts packed one after another, without the KV pool: TokenLogprobs of every
+        prompt's tokens after its first, in order, on the device. With alternatives (top_k > 0) the logits exist
+        for SCORE_ROWS rows at a time, without them not at all."""
+        from ..ops.logprobs import TokenLogprobs, head_logprobs, token_logprobs
+        lens = [len(p) for p in prompts]
+        T = sum(lens)
+        bounds = np.concatenate([[0], np.cumsum(lens)]).astype(np.int32)
+        ids = np.concatenate([np.asarray(p, np.int64) for p in prompts])
+        pos = np.concatenate([np.arange(n, dtype=np.int64) for n in lens])
+        last = np.zeros(T, bool)
+        last[bounds[1:] - 1] = True
+        rows = np.flatnonzero(~last)  # every token but each prompt's last predicts its successor
+        dev = self.device
+        ids_d, pos_d, rows_d = (torch.from_numpy(a).to(dev) for a in (ids, pos, rows))
+        fb = ForwardBatch(mode=ForwardMode.EXTEND, batch_size=len(lens), num_tokens=T, input_ids=ids_d,
+                          positions=pos_d, out_cache_loc=None, seq_lens=None, block_table=None, logits_idx=rows_d,
+                          qo_indptr=torch.from_numpy(bounds).to(dev), max_extend=max(lens), max_seq_len=max(lens),
+                          packed_prompts=True)
+        h = self.model(fb)
+        want = ids_d.index_select(0, rows_d + 1)
+        V, off = self.vocab_valid, self.vocab_start
+        if V == 0:  # a shard past the vocabulary's end
+            none = torch.full((len(rows),), float("-inf"), dtype=torch.float32, device=dev)
+            local = TokenLogprobs(none, torch.zeros_like(none), none, none[:, None].expand(-1, top_k),
+                                  torch.zeros(len(rows), top_k, dtype=torch.int64, device=dev))
+        elif top_k == 0:
+            local = head_logprobs(h, self.model.lm_head.gemm_weight, want, vocab_offset=off, valid_vocab=V)
+        else:
+            k = min(top_k, V)
+            parts = [token_logprobs(self.model.compute_logits(h[a:a + self.SCORE_ROWS]), want[a:a + self.SCORE_ROWS],
+                                    top_k=k, vocab_offset=off, valid_vocab=V)
+                     for a in range(0, len(rows), self.SCORE_ROWS)]
+            local = TokenLogprobs(*(torch.cat(t) for t in zip(*parts)))
+            if k < top_k:  # a shard smaller than the alternatives asked for
+                fill = torch.full((len(rows), top_k - k), float("-inf"), device=dev)
+                local = local._replace(top_logprobs=torch.cat([local.top_logprobs, fill], 1),
+                                       top_ids=torch.cat([local.top_ids, torch.zeros_like(fill, dtype=torch.int64)], 1))
+        return self._merge_scores(local, top_k)
+
+    def _merge_scores(self, local, top_k: int):
+        """The vocabulary shards' statistics gathered and joined (ids travel as fp32: exact below 2^24)."""
+        tp = get_state().tp_size
+        if tp == 1:
+            return local
+        from ..ops.logprobs import TokenLogprobs, merge_shards
+        pack = torch.cat([local.logprobs[:, None], local.entropy[:, None], local.lse[:, None], local.top_logprobs,
+                          local.top_ids.float()], dim=1).contiguous()
+        g = torch.empty(tp * pack.shape[0], pack.shape[1], dtype=torch.float32, device=pack.device)
+        tp_all_gather_into(g, pack)
+        k = top_k
+        return merge_shards([TokenLogprobs(s[:, 0], s[:, 1], s[:, 2], s[:, 3:3 + k], s[:, 3 + k:].long())
+                             for s in g.view(tp, pack.shape[0], -1)])
+
     def apply_page_updates(self, upd: torch.Tensor) -> None:
         """upd: [U*3] int32 (req_slot, page_index, page_id) triples."""
         if upd.numel() == 0:

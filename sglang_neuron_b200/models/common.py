@@ -26,6 +26,7 @@ from ..model_executor.forward_batch import ForwardBatch, ForwardMode
 from ..ops import activation as act_ops
 from ..ops import moe as moe_ops
 from ..ops.norm import fused_add_rmsnorm, rmsnorm
+from ..ops.prompt import prompt_attention
 from ..ops.rope import build_cos_sin_cache, rope_qk_norm_kv_write
 from ..parallel.collectives import (FusedNorm, deferred_reduction, dp_gather_rows, dp_scatter_rows,
                                     fused_combine_all_reduce, pp_isend_hidden, pp_recv_hidden, pp_send_hidden,
@@ -101,6 +102,15 @@ class GQAAttention(nn.Module):
         q = qkv[:, :qs]
         k = qkv[:, qs:qs + kvs]
         v = qkv[:, qs + kvs:]
+        if fb.packed_prompts:
+            # whole prompts that leave no cache behind: attention straight over this step's keys and values
+            rope_qk_norm_kv_write(q, k, v, fb.positions, self.cos_sin, self.num_heads, self.num_kv_heads,
+                                  self.head_dim, self.cfg.rot_dim, self.cfg.rope_neox,
+                                  self.q_norm.weight if self.q_norm is not None else None,
+                                  self.k_norm.weight if self.k_norm is not None else None, self.cfg.rms_norm_eps)
+            o = prompt_attention(q, k, v, fb.qo_indptr, self.num_heads, self.num_kv_heads, self.head_dim,
+                                 window=self.window, sm_scale=self.scaling, sinks=self.sinks_f32())
+            return self.o_proj(o, norm=norm)
         kc, vc = self.kv_cache()
         if self.window > 0 and self.kv_pool.swa is not None:
             fb = self.kv_pool.swa.batch(fb)  # block table and write slots in window-pool pages

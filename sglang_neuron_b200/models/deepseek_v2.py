@@ -18,6 +18,7 @@ from torch import nn
 from ..layers.linear import ColumnParallelLinear, ReplicatedLinear, RowParallelLinear
 from ..model_executor.forward_batch import ForwardBatch
 from ..ops.mla import mla_attention, mla_write_rows
+from ..ops.prompt import prompt_attention
 from ..ops.rope import apply_rope_ref, yarn_get_mscale
 from ..parallel.state import get_state
 from .common import CausalLM, DecoderLayer, DenseMLP, MoEBlock, RMSNorm, RotaryCache
@@ -98,7 +99,27 @@ class MLAAttention(nn.Module):
                             0, 0)
         return self.o_proj(o, norm=norm)
 
+    def _forward_prompts(self, h: torch.Tensor, fb: ForwardBatch, norm=None) -> torch.Tensor:
+        """Whole prompts without the latent pool: keys and values decompressed from the latent rows (k_nope and v of
+        every head in one product each) and plain multi-head attention, nope + rope wide keys, v_head_dim values."""
+        T, H = h.shape[0], self.num_heads
+        q = self.q_proj(h).view(T, H, self.nope + self.rope)
+        kv_a = self.kv_a_proj(h)
+        c = self.kv_a_layernorm(kv_a[:, : self.r].contiguous())
+        k = torch.empty_like(q)
+        k[:, :, : self.nope] = torch.nn.functional.linear(c, self.w_uk.view(H * self.nope, self.r)).view(T, H, self.nope)
+        k[:, :, self.nope:] = apply_rope_ref(kv_a[:, None, self.r:], fb.positions, self.cos_sin, self.rope,
+                                             False).to(h.dtype)
+        q[:, :, self.nope:] = apply_rope_ref(q[:, :, self.nope:], fb.positions, self.cos_sin, self.rope,
+                                             False).to(h.dtype)
+        v = torch.nn.functional.linear(c, self.w_uv.view(H * self.vd, self.r))
+        o = prompt_attention(q.view(T, -1), k.view(T, -1), v, fb.qo_indptr, H, H, self.nope + self.rope,
+                             v_head_dim=self.vd, sm_scale=self.scaling)
+        return self.o_proj(o, norm=norm)
+
     def forward(self, h: torch.Tensor, fb: ForwardBatch, norm=None) -> torch.Tensor:
+        if fb.packed_prompts:
+            return self._forward_prompts(h, fb, norm)
         if self._native(h):
             return self._forward_native(h, fb, norm)
         T = h.shape[0]
