@@ -8,6 +8,7 @@
 #include "../common.cuh"
 #include "../tma_host.h"
 #include <algorithm>
+#include <type_traits>
 
 namespace {
 
@@ -50,6 +51,8 @@ struct PromptParams {
   const float* sinks;
   int T, B, heads, kv_heads, window;
   float scale;  // of the scores, in log2 units
+  int pair_heads, pairs, items;
+  uint32_t idesc;  // the operands' type, for the MMA
 };
 
 SNB_DEVICE int seq_bound(const PromptParams& p, int b) { return min(max(__ldg(p.indptr + b), 0), p.T); }
@@ -118,36 +121,424 @@ __device__ __noinline__ void attend_row(const PromptParams& p, int first, int t,
   for (int d = 0; d < DV / 32; d += 2) *reinterpret_cast<uint32_t*>(dst + d) = pack2<T>(o[d] * r, o[d + 1] * r);
 }
 
-template <typename T, int D, int DV>
-__global__ void __launch_bounds__(128) prompt_attention_rows_kernel(const PromptParams p) {
-  snb::pdl_wait();
-  snb::pdl_trigger();
-  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int t = (int)(w / p.heads), h = (int)(w % p.heads);
-  if (t >= p.T) return;
-  int lo = 0, hi = p.B;  // the last b with bound(b) <= t
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (seq_bound(p, mid) <= t) lo = mid;
-    else hi = mid;
+// ---- tensor-core kernel ---------------------------------------------------------------------------------------
+constexpr int BQ = 128;  // query rows of a tile: one tensor-memory lane and one softmax thread each
+constexpr int BKV = 128;  // keys of a block
+constexpr int CHUNK = 128 * 128;  // bytes of 128 rows x 64 16-bit elements (one swizzled TMA box)
+constexpr int THREADS = 320;      // 2 x 4 softmax warps, a load warp, an MMA warp
+
+template <int D, int DV>
+struct Cfg {
+  static constexpr int QB = D / 64 * CHUNK, KB = D / 64 * CHUNK, VB = DV / 64 * CHUNK;
+  static constexpr int NK = D == 64 ? 4 : D == 128 ? 3 : 2, NV = D == 64 ? 4 : D == 128 ? 2 : 1;
+  static constexpr int SMEM = 2 * QB + NK * KB + NV * VB + 1024 + 512;
+};
+
+// D[tmem] (+)= A[tmem] B[smem]: A holds two 16-bit values per 32-bit column
+SNB_DEVICE void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc));
+}
+SNB_DEVICE void tmem_st_x32(uint32_t at, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
+      "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
+      "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(at)
+      : "memory");
+}
+SNB_DEVICE void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// B operand whose rows (keys) are the contraction: 64-wide column chunks `CHUNK` bytes apart, 8-row groups 1024 apart
+SNB_DEVICE uint64_t desc_v(uint32_t saddr) {
+  return (uint64_t)((saddr & 0x3FFFF) >> 4) | (uint64_t)(CHUNK >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 |
+         (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+
+// A work item: two query tiles that share their keys and values. With an even group size they are two heads of one
+// group over the same 128 tokens, otherwise 256 consecutive tokens of one head.
+struct Item {
+  int first, len;  // the prompt's first token and length
+  int r0;          // first query row, counted from `first`
+  int h0;          // head of the first tile
+  int kb0, kb1;    // key blocks [kb0, kb1), counted from `first`
+};
+
+// Item w of the list (tile, head pair): the prompts in order, each prompt's tiles from its last one down. Called by
+// whole warps. False past the end.
+SNB_DEVICE bool decode_item(const PromptParams& p, int w, Item& it) {
+  const int lane = threadIdx.x & 31;
+  const int rows = p.pair_heads ? BQ : 2 * BQ;
+  int idx = w / p.pairs;
+  const int pair = w % p.pairs;
+  for (int b0 = 0; b0 < p.B; b0 += 32) {
+    const int b = b0 + lane;
+    int a = 0, n = 0;
+    if (b < p.B) {
+      a = seq_bound(p, b);
+      n = max(0, seq_bound(p, b + 1) - a);
+    }
+    const int nt = (n + rows - 1) / rows;
+    int incl = nt;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += up;
+    }
+    const unsigned in = __ballot_sync(0xffffffffu, incl > idx);
+    if (in) {
+      const int src = __ffs(in) - 1;
+      it.first = __shfl_sync(0xffffffffu, a, src);
+      it.len = __shfl_sync(0xffffffffu, n, src);
+      it.r0 = (__shfl_sync(0xffffffffu, incl, src) - 1 - idx) * rows;
+      it.h0 = p.pair_heads ? pair * 2 : pair;
+      it.kb1 = (min(it.len, it.r0 + rows) + BKV - 1) / BKV;
+      it.kb0 = p.window > 0 ? max(0, it.r0 - p.window + 1) / BKV : 0;
+      return true;
+    }
+    idx -= __shfl_sync(0xffffffffu, incl, 31);
   }
-  const int first = seq_bound(p, lo);
-  if (t < first || t >= seq_bound(p, lo + 1)) return;
-  attend_row<T, D, DV>(p, first, t, h);
+  return false;
 }
 
 template <typename T, int D, int DV>
-void launch(const PromptParams& p, cudaStream_t st) {
-  const int64_t warps = (int64_t)p.T * p.heads;
-  C10_CUDA_CHECK(snb::launch_pdl(prompt_attention_rows_kernel<T, D, DV>, dim3((unsigned)((warps + 3) / 4)), dim3(128),
-                                 0, st, p));
+__global__ void __launch_bounds__(THREADS, 1)
+    prompt_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
+                            const __grid_constant__ CUtensorMap tv, const __grid_constant__ PromptParams p,
+                            int* status) {
+  using C = Cfg<D, DV>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sQ = smem;
+  uint8_t* sK = sQ + 2 * C::QB;
+  uint8_t* sV = sK + C::NK * C::KB;
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(sV + C::NV * C::VB);
+  uint64_t* q_empty = q_full + 1;
+  uint64_t* k_full = q_empty + 1;
+  uint64_t* k_empty = k_full + C::NK;
+  uint64_t* v_full = k_empty + C::NK;
+  uint64_t* v_empty = v_full + C::NV;
+  uint64_t* s_full = v_empty + C::NV;  // [2] scores of a tile are in tensor memory
+  uint64_t* p_full = s_full + 2;       // [2] a tile's weights are, and its output is rescaled
+  uint64_t* o_full = p_full + 2;       // [2] a tile's output has taken up a block
+  uint64_t* drain = o_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  int* issued = reinterpret_cast<int*>(tmem_slot + 1);  // loads issued: q, k, v
+  int* taken = issued + 3;                              // and waited for
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    snb::mbar_init(q_full, 1);
+    snb::mbar_init(q_empty, 1);
+    for (int i = 0; i < C::NK; ++i) snb::mbar_init(&k_full[i], 1), snb::mbar_init(&k_empty[i], 1);
+    for (int i = 0; i < C::NV; ++i) snb::mbar_init(&v_full[i], 1), snb::mbar_init(&v_empty[i], 1);
+    for (int j = 0; j < 2; ++j) {
+      snb::mbar_init(&s_full[j], 1);
+      snb::mbar_init(&p_full[j], 128);
+      snb::mbar_init(&o_full[j], 1);
+    }
+    snb::mbar_init(drain, 1);
+    for (int i = 0; i < 6; ++i) issued[i] = 0;
+    snb::fence_mbar_init();
+  }
+  if (warp == 9) {
+    snb::tmem_alloc(tmem_slot, 512);
+    snb::tmem_relinquish();
+  }
+  snb::tc_fence_before();
+  __syncthreads();
+  snb::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const uint32_t tS[2] = {tmem, tmem + 128}, tO[2] = {tmem + 256, tmem + 256 + DV};
+  snb::pdl_trigger();
+  snb::pdl_wait();
+  const int G = p.heads / p.kv_heads;
+
+  if (warp == 8) {
+    int nq = 0, nk = 0, nv = 0;
+    bool ok = true;
+    Item it;
+    for (int w = blockIdx.x; ok && w < p.items; w += gridDim.x) {
+      if (!decode_item(p, w, it)) break;
+      if (lane == 0) {
+        const int hk = it.h0 / G;
+        auto load_k = [&](int kb) {
+          const int s = nk % C::NK;
+          if (!snb::mbar_wait_bounded(&k_empty[s], ((nk / C::NK) & 1) ^ 1, status, SNB_ERR_TIMEOUT_TMA)) return false;
+          snb::mbar_arrive_expect_tx(&k_full[s], C::KB);
+#pragma unroll
+          for (int c = 0; c < D / 64; ++c)
+            snb::tma_load_2d(sK + s * C::KB + c * CHUNK, &tk, &k_full[s], hk * D + c * 64, it.first + kb * BKV);
+          ++nk;
+          return true;
+        };
+        auto load_v = [&](int kb) {
+          const int s = nv % C::NV;
+          if (!snb::mbar_wait_bounded(&v_empty[s], ((nv / C::NV) & 1) ^ 1, status, SNB_ERR_TIMEOUT_TMA)) return false;
+          snb::mbar_arrive_expect_tx(&v_full[s], C::VB);
+#pragma unroll
+          for (int c = 0; c < DV / 64; ++c)
+            snb::tma_load_2d(sV + s * C::VB + c * CHUNK, &tv, &v_full[s], hk * DV + c * 64, it.first + kb * BKV);
+          ++nv;
+          return true;
+        };
+        ok = snb::mbar_wait_bounded(q_empty, (nq & 1) ^ 1, status, SNB_ERR_TIMEOUT_TMA);
+        if (ok) {
+          snb::mbar_arrive_expect_tx(q_full, 2 * C::QB);
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c)
+              snb::tma_load_2d(sQ + j * C::QB + c * CHUNK, &tq, q_full, (it.h0 + (p.pair_heads ? j : 0)) * D + c * 64,
+                               it.first + it.r0 + (p.pair_heads ? 0 : j * BQ));
+          ++nq;
+          for (int kb = it.kb0; ok && kb < it.kb1; ++kb) ok = load_k(kb) && load_v(kb);
+        }
+      }
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+    }
+    if (lane == 0) issued[0] = nq, issued[1] = nk, issued[2] = nv;
+  } else if (warp == 9) {
+    int nq = 0, nk = 0, nv = 0, np = 0;
+    bool ok = true;
+    Item it;
+    const uint32_t id_s = p.idesc | snb::idesc_bf16_f32(BQ, BKV) & ~(7u << 7 | 7u << 10);
+    const uint32_t id_o = p.idesc | snb::idesc_bf16_f32(BQ, DV) & ~(7u << 7 | 7u << 10) | 1u << 16;
+    for (int w = blockIdx.x; ok && w < p.items; w += gridDim.x) {
+      if (!decode_item(p, w, it)) break;
+      if (lane == 0) {
+        auto wait = [&](uint64_t* bar, int parity) {
+          const bool r = snb::mbar_wait_bounded(bar, parity, status, SNB_ERR_TIMEOUT_MMA);
+          snb::tc_fence_after();
+          return r;
+        };
+        auto scores = [&](int j, int s) {
+          const uint32_t a = snb::smem_u32(sQ + j * C::QB), b = snb::smem_u32(sK + s * C::KB);
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            const uint32_t off = (k / 4) * CHUNK + (k % 4) * 32;
+            snb::mma_bf16_ss(tS[j], snb::smem_desc_sw128(a + off), snb::smem_desc_sw128(b + off), id_s, k > 0);
+          }
+          snb::mma_commit(&s_full[j]);
+        };
+        auto output = [&](int j, int s, bool more) {
+          const uint32_t b = snb::smem_u32(sV + s * C::VB);
+#pragma unroll
+          for (int k = 0; k < BKV / 16; ++k)
+            mma_ts(tO[j], tS[j] + k * 8, desc_v(b + k * 2048), id_o, more || k > 0);
+          snb::mma_commit(&o_full[j]);
+        };
+        const int nb = it.kb1 - it.kb0;
+        ok = wait(q_full, nq & 1) && wait(&k_full[nk % C::NK], (nk / C::NK) & 1);
+        if (ok) {
+          scores(0, nk % C::NK);
+          scores(1, nk % C::NK);
+          snb::mma_commit(&k_empty[nk % C::NK]);
+          ++nk;
+          if (nb == 1) snb::mma_commit(q_empty);
+        }
+        for (int i = 0; ok && i < nb; ++i) {
+          const bool next = i + 1 < nb;
+          const int ks = nk % C::NK, vs = nv % C::NV;
+          ok = (!next || wait(&k_full[ks], (nk / C::NK) & 1)) && wait(&v_full[vs], (nv / C::NV) & 1);
+          for (int j = 0; ok && j < 2; ++j) {
+            ok = wait(&p_full[j], np & 1);
+            if (!ok) break;
+            output(j, vs, i > 0);
+            if (next) scores(j, ks);
+          }
+          if (!ok) break;
+          snb::mma_commit(&v_empty[vs]);
+          ++nv;
+          ++np;
+          if (next) {
+            snb::mma_commit(&k_empty[ks]);
+            ++nk;
+            if (i + 2 == nb) snb::mma_commit(q_empty);
+          }
+        }
+        ++nq;
+      }
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+    }
+    if (lane == 0) {
+      taken[0] = nq, taken[1] = nk, taken[2] = nv;
+      if (!ok) {  // products in flight still read this CTA's memory
+        snb::mma_commit(drain);
+        snb::mbar_wait_bounded(drain, 0, status, SNB_ERR_TIMEOUT_MMA);
+      }
+    }
+  } else {
+    const int j = warp >> 2;  // this warpgroup's tile
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_at = tS[j] + lanes, o_at = tO[j] + lanes;
+    const int row = (warp & 3) * 32 + lane;
+    int ns = 0;  // blocks done by this tile, over all items
+    bool ok = true;
+    Item it;
+    auto wait = [&](uint64_t* bar, int parity) {
+      const bool r = snb::mbar_wait_bounded(bar, parity, status, SNB_ERR_TIMEOUT_EPI);
+      snb::tc_fence_after();
+      return __all_sync(0xffffffffu, r) != 0;
+    };
+    for (int w = blockIdx.x; ok && w < p.items; w += gridDim.x) {
+      if (!decode_item(p, w, it)) break;
+      const int head = it.h0 + (p.pair_heads ? j : 0);
+      const int r0 = it.r0 + (p.pair_heads ? 0 : j * BQ);
+      const int rel = r0 + row;  // this thread's query, counted from the prompt's first token
+      const int lo = p.window > 0 ? rel - p.window + 1 : 0;
+      float m = -INFINITY, l = 0.f;
+      for (int kb = it.kb0; ok && kb < it.kb1; ++kb, ++ns) {
+        ok = wait(&s_full[j], ns & 1);
+        if (!ok) break;
+        uint32_t s[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) snb::tmem_ld_32x32b_x32(s_at + c * 32, s[c]);
+        snb::tmem_ld_wait();
+        const int k0 = kb * BKV;
+        if (k0 + BKV - 1 > r0 || (p.window > 0 && k0 < r0 + BQ - p.window)) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const int key = k0 + c * 32 + i;
+              if (key > rel || key < lo) s[c][i] = 0xff800000u;
+            }
+        }
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) mx[c] = fmaxf(mx[c], __uint_as_float(s[c][i]));
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        // The reference follows the maximum only when that has risen by more than 2^8: weights stay below 2^8, and
+        // the output in tensor memory is rarely read and written for it.
+        if (__any_sync(0xffffffffu, (top - m) * p.scale > 8.f || (m == -INFINITY && top > m))) {
+          const float mn = fmaxf(m, top);
+          const float f = mn == -INFINITY ? 1.f : ex2((m - mn) * p.scale);
+          l *= f;
+          m = mn;
+          if (kb > it.kb0) {
+            ok = wait(&o_full[j], (ns - 1) & 1);
+            if (!ok) break;
+#pragma unroll 1
+            for (int c = 0; c < DV / 32; ++c) {
+              uint32_t o[32];
+              snb::tmem_ld_32x32b_x32(o_at + c * 32, o);
+              snb::tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+              tmem_st_x32(o_at + c * 32, o);
+            }
+          }
+        }
+        const float ref = m == -INFINITY ? 0.f : m * p.scale;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < 4; c += 2) {
+          uint32_t w2[32];
+#pragma unroll
+          for (int d = 0; d < 2; ++d)
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              const float a = ex2(fmaf(__uint_as_float(s[c + d][i]), p.scale, -ref));
+              const float b = ex2(fmaf(__uint_as_float(s[c + d][i + 1]), p.scale, -ref));
+              sum[2 * d] += a;
+              sum[2 * d + 1] += b;
+              w2[d * 16 + i / 2] = pack2<T>(a, b);
+            }
+          tmem_st_x32(s_at + c * 16, w2);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tmem_st_wait();
+        snb::tc_fence_before();
+        snb::mbar_arrive(&p_full[j]);
+      }
+      if (!ok) break;
+      ok = wait(&o_full[j], (ns - 1) & 1);
+      if (!ok) break;
+      if (p.sinks != nullptr) l += ex2(p.sinks[head] * LOG2E - (m == -INFINITY ? 0.f : m * p.scale));
+      const float r = l > 0.f || l != l ? 1.f / l : 0.f;
+      const bool store = rel < it.len;
+      const int t = it.first + rel;
+      T* dst = reinterpret_cast<T*>(p.out) + (int64_t)t * p.os + (int64_t)head * DV;
+      bool odd = false;
+#pragma unroll
+      for (int c = 0; c < DV / 32; ++c) {
+        uint32_t o[32];
+        snb::tmem_ld_32x32b_x32(o_at + c * 32, o);
+        snb::tmem_ld_wait();
+        uint32_t w2[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float a = __uint_as_float(o[2 * i]) * r, b = __uint_as_float(o[2 * i + 1]) * r;
+          odd |= !(fabsf(a) < INFINITY) || !(fabsf(b) < INFINITY);
+          w2[i] = pack2<T>(a, b);
+        }
+        if (store)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<uint4*>(dst + c * 32 + i * 8) =
+                make_uint4(w2[4 * i], w2[4 * i + 1], w2[4 * i + 2], w2[4 * i + 3]);
+      }
+      // A NaN or infinity in a masked value still meets a weight of 0 in the product (0 * inf = NaN): rows that came
+      // out so are computed once more without touching what is masked.
+      unsigned again = __ballot_sync(0xffffffffu, odd && store);
+      while (again) {
+        const int src = __ffs(again) - 1;
+        again &= again - 1;
+        attend_row<T, D, DV>(p, it.first, it.first + r0 + (warp & 3) * 32 + src, head);
+      }
+    }
+  }
+  snb::tc_fence_before();
+  __syncthreads();
+  if (warp == 8 && lane == 0) {
+    // a CTA that stopped early still waits (bounded) for the loads it issued
+    if (taken[0] < issued[0]) snb::mbar_wait_bounded(q_full, taken[0] & 1, status, SNB_ERR_TIMEOUT_TMA);
+    for (int i = taken[1]; i < issued[1]; ++i)
+      if (!snb::mbar_wait_bounded(&k_full[i % C::NK], (i / C::NK) & 1, status, SNB_ERR_TIMEOUT_TMA)) break;
+    for (int i = taken[2]; i < issued[2]; ++i)
+      if (!snb::mbar_wait_bounded(&v_full[i % C::NV], (i / C::NV) & 1, status, SNB_ERR_TIMEOUT_TMA)) break;
+  }
+  if (warp == 9) snb::tmem_dealloc(tmem, 512);
+}
+
+template <typename T, int D, int DV>
+void launch(PromptParams p, int* status, cudaStream_t st) {
+  using C = Cfg<D, DV>;
+  constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+  const auto dt = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  auto map = [&](const void* base, int64_t width, int64_t stride) {
+    return snb_host::make_tmap_2d(base, dt, width, p.T, stride * 2, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+  };
+  const CUtensorMap tq = map(p.q, (int64_t)p.heads * D, p.qs), tk = map(p.k, (int64_t)p.kv_heads * D, p.ks),
+                    tv = map(p.v, (int64_t)p.kv_heads * DV, p.vs);
+  p.idesc = bf16 ? 1u << 7 | 1u << 10 : 0u;
+  p.pair_heads = (p.heads / p.kv_heads) % 2 == 0;
+  p.pairs = p.pair_heads ? p.heads / 2 : p.heads;
+  const int rows = p.pair_heads ? BQ : 2 * BQ;
+  const int64_t items = ((int64_t)p.T / rows + std::min(p.B, p.T)) * p.pairs;  // at most one ragged tile per prompt
+  TORCH_CHECK(items < (int64_t(1) << 31), "prompt_attention: too much work for one call");
+  p.items = (int)items;
+  auto kern = prompt_attention_kernel<T, D, DV>;
+  C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+  const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+  C10_CUDA_CHECK(snb::launch_pdl(kern, dim3(std::min(p.items, sms)), dim3(THREADS), C::SMEM, st, tq, tk, tv, p,
+                                 status));
 }
 
 template <typename T>
-void dispatch(const PromptParams& p, int64_t D, int64_t DV, cudaStream_t st) {
-  if (D == 64 && DV == 64) launch<T, 64, 64>(p, st);
-  else if (D == 128 && DV == 128) launch<T, 128, 128>(p, st);
-  else if (D == 192 && DV == 128) launch<T, 192, 128>(p, st);
+void dispatch(const PromptParams& p, int64_t D, int64_t DV, int* status, cudaStream_t st) {
+  if (D == 64 && DV == 64) launch<T, 64, 64>(p, status, st);
+  else if (D == 128 && DV == 128) launch<T, 128, 128>(p, status, st);
+  else if (D == 192 && DV == 128) launch<T, 192, 128>(p, status, st);
   else TORCH_CHECK(false, "prompt_attention: head dims ", D, " / ", DV, " (64 / 64, 128 / 128 or 192 / 128)");
 }
 
@@ -199,7 +590,7 @@ void prompt_attention(at::Tensor out, at::Tensor q, at::Tensor k, at::Tensor v, 
   p.window = (int)std::min<int64_t>(std::max<int64_t>(window, 0), T);
   p.scale = (float)(sm_scale * 1.4426950408889634);
   auto st = at::cuda::getCurrentCUDAStream();
-  if (dt == at::kBFloat16) dispatch<__nv_bfloat16>(p, D, DV, st);
-  else if (dt == at::kHalf) dispatch<__half>(p, D, DV, st);
+  if (dt == at::kBFloat16) dispatch<__nv_bfloat16>(p, D, DV, status.data_ptr<int>(), st);
+  else if (dt == at::kHalf) dispatch<__half>(p, D, DV, status.data_ptr<int>(), st);
   else TORCH_CHECK(false, "prompt_attention: dtype ", dt);
 }
