@@ -12,6 +12,10 @@
 
 namespace {
 
+#ifndef EMULATE_N
+#define EMULATE_N 4
+#endif
+constexpr int EMULATE = EMULATE_N;  // one pair of exponentials in this many runs on the FMA pipe
 constexpr float LOG2E = 1.4426950408889634f;
 
 SNB_DEVICE float ex2(float x) {
@@ -41,6 +45,69 @@ template <>
 SNB_DEVICE uint32_t pack2<__half>(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// two fp32 values in one 64-bit register pair: one issue slot for both
+SNB_DEVICE uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+SNB_DEVICE float2 split(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+SNB_DEVICE uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+SNB_DEVICE uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+SNB_DEVICE float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+SNB_DEVICE float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+SNB_DEVICE float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// 2^x of two values on the FMA pipe: x = n + f with n the nearest integer (found by adding 1.5 * 2^23) and |f| <= 1/2,
+// 2^f by the cubic whose largest relative error on that interval is least (7.5e-5, by Remez exchange; weights are
+// rounded to 2^-9 or 2^-12 next), n added to the exponent. Below -125 the result is 2^-125; 128 and above (`HIGH`: x
+// can get there) and NaN become values past every 16-bit type's range.
+template <bool HIGH>
+SNB_DEVICE float2 exp2_fma(uint64_t x) {
+  float2 c = split(x);
+  c.x = max_nan(c.x, -125.f);
+  c.y = max_nan(c.y, -125.f);
+  if (HIGH) {
+    c.x = min_nan(c.x, 128.f);
+    c.y = min_nan(c.y, 128.f);
+  }
+  x = pair(c.x, c.y);
+  const uint64_t big = pair(12582912.f, 12582912.f), less = pair(-12582912.f, -12582912.f);
+  const uint64_t n = add2(x, big);
+  const uint64_t f = fma2(add2(n, less), pair(-1.f, -1.f), x);
+  uint64_t y = fma2(pair(0.05517166852953102f, 0.05517166852953102f), f, pair(0.2426111251115799f, 0.2426111251115799f));
+  y = fma2(y, f, pair(0.6932609677314758f, 0.6932609677314758f));
+  y = fma2(y, f, pair(0.9999280571937561f, 0.9999280571937561f));
+  const float2 ny = split(n), r = split(y);
+  return make_float2(__int_as_float(__float_as_int(r.x) + (__float_as_int(ny.x) << 23)),
+                     __int_as_float(__float_as_int(r.y) + (__float_as_int(ny.y) << 23)));
 }
 
 struct PromptParams {
@@ -125,14 +192,27 @@ __device__ __noinline__ void attend_row(const PromptParams& p, int first, int t,
 constexpr int BQ = 128;  // query rows of a tile: one tensor-memory lane and one softmax thread each
 constexpr int BKV = 128;  // keys of a block
 constexpr int CHUNK = 128 * 128;  // bytes of 128 rows x 64 16-bit elements (one swizzled TMA box)
-constexpr int THREADS = 320;      // 2 x 4 softmax warps, a load warp, an MMA warp
+constexpr int LOAD_WARP = 16, MMA_WARP = 17;
+constexpr int THREADS = 18 * 32;  // 2 tiles x 2 halves of the keys x 4 softmax warps, a load warp, an MMA warp
 
 template <int D, int DV>
 struct Cfg {
   static constexpr int QB = D / 64 * CHUNK, KB = D / 64 * CHUNK, VB = DV / 64 * CHUNK;
   static constexpr int NK = D == 64 ? 4 : D == 128 ? 3 : 2, NV = D == 64 ? 4 : D == 128 ? 2 : 1;
-  static constexpr int SMEM = 2 * QB + NK * KB + NV * VB + 1024 + 512;
+  static constexpr int SMEM = 2 * QB + NK * KB + NV * VB + 2 * BQ * 4 + 1024 + 512;
 };
+
+// One lane of a converged warp; the compiler keeps what such a branch uses in uniform registers, which the MMA's
+// operands have to be in (converting them costs more than the 64 cycles that an MMA takes).
+SNB_DEVICE bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r != 0;
+}
 
 // D[tmem] (+)= A[tmem] B[smem]: A holds two 16-bit values per 32-bit column
 SNB_DEVICE void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
@@ -152,6 +232,32 @@ SNB_DEVICE void tmem_st_x32(uint32_t at, const uint32_t (&r)[32]) {
       "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
       "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(at)
       : "memory");
+}
+SNB_DEVICE void tmem_st_x8(uint32_t at, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::"r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(at)
+               : "memory");
+}
+SNB_DEVICE void tmem_ld_x16(uint32_t at, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(at));
+}
+// Named barriers of the two warps that share a quarter of a tile's rows (64 threads)
+SNB_DEVICE void bar_pair(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
+SNB_DEVICE bool bar_or(int id, bool v) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %2, 0;\n\t"
+      "bar.red.or.pred q, %1, 64, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(id), "r"((uint32_t)v)
+      : "memory");
+  return r != 0;
 }
 SNB_DEVICE void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -207,6 +313,14 @@ SNB_DEVICE bool decode_item(const PromptParams& p, int w, Item& it) {
   return false;
 }
 
+// This CTA's r-th item. The list's items shrink slowly (a prompt's tiles come last tile first), so the CTAs take them
+// in alternating order: 0..n-1, then n-1..0.
+SNB_DEVICE bool next_item(const PromptParams& p, int r, Item& it) {
+  const int n = gridDim.x;
+  const int64_t w = (int64_t)r * n + ((r & 1) ? n - 1 - blockIdx.x : blockIdx.x);
+  return w < p.items && decode_item(p, (int)w, it);
+}
+
 template <typename T, int D, int DV>
 __global__ void __launch_bounds__(THREADS, 1)
     prompt_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
@@ -225,14 +339,15 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint64_t* v_full = k_empty + C::NK;
   uint64_t* v_empty = v_full + C::NV;
   uint64_t* s_full = v_empty + C::NV;  // [2] scores of a tile are in tensor memory
-  uint64_t* p_full = s_full + 2;       // [2] a tile's weights are, and its output is rescaled
-  uint64_t* o_full = p_full + 2;       // [2] a tile's output has taken up a block
+  uint64_t* p_full = s_full + 2;       // [2][2] the first / second half of a tile's weights are (its output rescaled)
+  uint64_t* o_full = p_full + 4;       // [2] a tile's output has taken up a block
   uint64_t* drain = o_full + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   int* issued = reinterpret_cast<int*>(tmem_slot + 1);  // loads issued: q, k, v
   int* taken = issued + 3;                              // and waited for
+  float* sX = reinterpret_cast<float*>(taken + 3);      // [2][128] what the two halves of a row exchange
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     snb::mbar_init(q_full, 1);
     snb::mbar_init(q_empty, 1);
@@ -240,14 +355,15 @@ __global__ void __launch_bounds__(THREADS, 1)
     for (int i = 0; i < C::NV; ++i) snb::mbar_init(&v_full[i], 1), snb::mbar_init(&v_empty[i], 1);
     for (int j = 0; j < 2; ++j) {
       snb::mbar_init(&s_full[j], 1);
-      snb::mbar_init(&p_full[j], 128);
+      snb::mbar_init(&p_full[2 * j], 8);
+      snb::mbar_init(&p_full[2 * j + 1], 8);
       snb::mbar_init(&o_full[j], 1);
     }
     snb::mbar_init(drain, 1);
     for (int i = 0; i < 6; ++i) issued[i] = 0;
     snb::fence_mbar_init();
   }
-  if (warp == 9) {
+  if (warp == MMA_WARP) {
     snb::tmem_alloc(tmem_slot, 512);
     snb::tmem_relinquish();
   }
@@ -255,17 +371,15 @@ __global__ void __launch_bounds__(THREADS, 1)
   __syncthreads();
   snb::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const uint32_t tS[2] = {tmem, tmem + 128}, tO[2] = {tmem + 256, tmem + 256 + DV};
   snb::pdl_trigger();
   snb::pdl_wait();
   const int G = p.heads / p.kv_heads;
 
-  if (warp == 8) {
+  if (warp == LOAD_WARP) {
     int nq = 0, nk = 0, nv = 0;
     bool ok = true;
     Item it;
-    for (int w = blockIdx.x; ok && w < p.items; w += gridDim.x) {
-      if (!decode_item(p, w, it)) break;
+    for (int r = 0; ok && next_item(p, r, it); ++r) {
       if (lane == 0) {
         const int hk = it.h0 / G;
         auto load_k = [&](int kb) {
@@ -304,180 +418,250 @@ __global__ void __launch_bounds__(THREADS, 1)
       ok = __shfl_sync(0xffffffffu, ok, 0);
     }
     if (lane == 0) issued[0] = nq, issued[1] = nk, issued[2] = nv;
-  } else if (warp == 9) {
+  } else if (warp == MMA_WARP) {
     int nq = 0, nk = 0, nv = 0, np = 0;
     bool ok = true;
     Item it;
     const uint32_t id_s = p.idesc | snb::idesc_bf16_f32(BQ, BKV) & ~(7u << 7 | 7u << 10);
     const uint32_t id_o = p.idesc | snb::idesc_bf16_f32(BQ, DV) & ~(7u << 7 | 7u << 10) | 1u << 16;
-    for (int w = blockIdx.x; ok && w < p.items; w += gridDim.x) {
-      if (!decode_item(p, w, it)) break;
-      if (lane == 0) {
-        auto wait = [&](uint64_t* bar, int parity) {
-          const bool r = snb::mbar_wait_bounded(bar, parity, status, SNB_ERR_TIMEOUT_MMA);
-          snb::tc_fence_after();
-          return r;
-        };
-        auto scores = [&](int j, int s) {
-          const uint32_t a = snb::smem_u32(sQ + j * C::QB), b = snb::smem_u32(sK + s * C::KB);
-#pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            const uint32_t off = (k / 4) * CHUNK + (k % 4) * 32;
-            snb::mma_bf16_ss(tS[j], snb::smem_desc_sw128(a + off), snb::smem_desc_sw128(b + off), id_s, k > 0);
-          }
-          snb::mma_commit(&s_full[j]);
-        };
-        auto output = [&](int j, int s, bool more) {
-          const uint32_t b = snb::smem_u32(sV + s * C::VB);
-#pragma unroll
-          for (int k = 0; k < BKV / 16; ++k)
-            mma_ts(tO[j], tS[j] + k * 8, desc_v(b + k * 2048), id_o, more || k > 0);
-          snb::mma_commit(&o_full[j]);
-        };
-        const int nb = it.kb1 - it.kb0;
-        ok = wait(q_full, nq & 1) && wait(&k_full[nk % C::NK], (nk / C::NK) & 1);
-        if (ok) {
-          scores(0, nk % C::NK);
-          scores(1, nk % C::NK);
-          snb::mma_commit(&k_empty[nk % C::NK]);
-          ++nk;
-          if (nb == 1) snb::mma_commit(q_empty);
-        }
-        for (int i = 0; ok && i < nb; ++i) {
-          const bool next = i + 1 < nb;
-          const int ks = nk % C::NK, vs = nv % C::NV;
-          ok = (!next || wait(&k_full[ks], (nk / C::NK) & 1)) && wait(&v_full[vs], (nv / C::NV) & 1);
-          for (int j = 0; ok && j < 2; ++j) {
-            ok = wait(&p_full[j], np & 1);
-            if (!ok) break;
-            output(j, vs, i > 0);
-            if (next) scores(j, ks);
-          }
-          if (!ok) break;
-          snb::mma_commit(&v_empty[vs]);
-          ++nv;
-          ++np;
-          if (next) {
-            snb::mma_commit(&k_empty[ks]);
-            ++nk;
-            if (i + 2 == nb) snb::mma_commit(q_empty);
-          }
-        }
-        ++nq;
-      }
-      ok = __shfl_sync(0xffffffffu, ok, 0);
-    }
-    if (lane == 0) {
-      taken[0] = nq, taken[1] = nk, taken[2] = nv;
-      if (!ok) {  // products in flight still read this CTA's memory
-        snb::mma_commit(drain);
-        snb::mbar_wait_bounded(drain, 0, status, SNB_ERR_TIMEOUT_MMA);
-      }
-    }
-  } else {
-    const int j = warp >> 2;  // this warpgroup's tile
-    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_at = tS[j] + lanes, o_at = tO[j] + lanes;
-    const int row = (warp & 3) * 32 + lane;
-    int ns = 0;  // blocks done by this tile, over all items
-    bool ok = true;
-    Item it;
+    const uint64_t q_desc = snb::smem_desc_sw128(snb::smem_u32(sQ)), k_desc = snb::smem_desc_sw128(snb::smem_u32(sK)),
+                   v_desc = desc_v(snb::smem_u32(sV));
     auto wait = [&](uint64_t* bar, int parity) {
-      const bool r = snb::mbar_wait_bounded(bar, parity, status, SNB_ERR_TIMEOUT_EPI);
+      const bool r = snb::mbar_wait_bounded(bar, parity, status, SNB_ERR_TIMEOUT_MMA);
       snb::tc_fence_after();
       return __all_sync(0xffffffffu, r) != 0;
     };
-    for (int w = blockIdx.x; ok && w < p.items; w += gridDim.x) {
-      if (!decode_item(p, w, it)) break;
+    // addresses in descriptors count 16-byte units
+    auto scores = [&](int j, int s) {
+      const uint64_t a = q_desc + j * (C::QB >> 4), b = k_desc + s * (C::KB >> 4);
+      if (elect_one()) {
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const int off = ((k / 4) * CHUNK + (k % 4) * 32) >> 4;
+          snb::mma_bf16_ss(tmem + j * 128, a + off, b + off, id_s, k > 0);
+        }
+        snb::mma_commit(&s_full[j]);
+      }
+    };
+    // Half `part` of a block's weights: keys 32 part .. 32 part + 31 of each half of the block
+    auto output = [&](int j, int s, int part, bool more) {
+      const uint64_t b = v_desc + s * (C::VB >> 4);
+      if (elect_one()) {
+#pragma unroll
+        for (int i = 0; i < BKV / 32; ++i) {
+          const int k = (i / 2) * 4 + part * 2 + i % 2;
+          mma_ts(tmem + 256 + j * DV, tmem + j * 128 + (k / 4) * 64 + (k % 4) * 8, b + k * (2048 >> 4), id_o,
+                 more || i > 0);
+        }
+        if (part) snb::mma_commit(&o_full[j]);
+      }
+    };
+    auto commit = [&](uint64_t* bar) {
+      if (elect_one()) snb::mma_commit(bar);
+    };
+    for (int r = 0; ok && next_item(p, r, it); ++r) {
+      const int nb = it.kb1 - it.kb0;
+      ok = wait(q_full, nq & 1) && wait(&k_full[nk % C::NK], (nk / C::NK) & 1);
+      if (ok) {
+        scores(0, nk % C::NK);
+        scores(1, nk % C::NK);
+        commit(&k_empty[nk % C::NK]);
+        ++nk;
+        if (nb == 1) commit(q_empty);
+      }
+      for (int i = 0; ok && i < nb; ++i) {
+        const bool next = i + 1 < nb;
+        const int ks = nk % C::NK, vs = nv % C::NV;
+        ok = (!next || wait(&k_full[ks], (nk / C::NK) & 1)) && wait(&v_full[vs], (nv / C::NV) & 1);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          ok = ok && wait(&p_full[2 * j], np & 1);
+          if (!ok) break;
+          output(j, vs, 0, i > 0);
+          ok = wait(&p_full[2 * j + 1], np & 1);
+          if (!ok) break;
+          output(j, vs, 1, true);
+          if (next) scores(j, ks);
+        }
+        if (!ok) break;
+        commit(&v_empty[vs]);
+        ++nv;
+        ++np;
+        if (next) {
+          commit(&k_empty[ks]);
+          ++nk;
+          if (i + 2 == nb) commit(q_empty);
+        }
+      }
+      ++nq;
+    }
+    if (lane == 0) taken[0] = nq, taken[1] = nk, taken[2] = nv;
+    if (!ok) {  // products in flight still read this CTA's memory
+      commit(drain);
+      snb::mbar_wait_bounded(drain, 0, status, SNB_ERR_TIMEOUT_MMA);
+    }
+  } else {
+    // Softmax: a row belongs to two threads, each with 64 of a block's 128 keys, in two warps of the same quarter of
+    // the tile's rows. Their scores lie in columns [64 h, 64 h + 64) of the tile's scores; their weights go over the
+    // first half of those.
+    const int j = warp >> 3, h = (warp >> 2) & 1, bar = 1 + j * 4 + (warp & 3);
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_at = tmem + j * 128 + h * 64 + lanes, o_at = tmem + 256 + j * DV + h * (DV / 2) + lanes;
+    const int row = (warp & 3) * 32 + lane;
+    float* x = sX + j * BQ + row;
+    int ns = 0;  // blocks done by this tile, over all items
+    bool ok = true;
+    Item it;
+    constexpr bool NARROW = std::is_same<T, __half>::value;
+    auto wait = [&](uint64_t* b, int parity) {
+      const bool r = snb::mbar_wait_bounded(b, parity, status, SNB_ERR_TIMEOUT_EPI);
+      snb::tc_fence_after();
+      return __all_sync(0xffffffffu, r) != 0;
+    };
+    // both halves get op(first half's v, second half's v)
+    auto exchange = [&](float v, auto op) {
+      if (h == 1) *x = v;
+      bar_pair(bar);
+      if (h == 0) *x = v = op(v, *x);
+      bar_pair(bar);
+      return h == 0 ? v : *x;
+    };
+    // A wait that ran out must end both warps of a pair at the same place: the pair agrees on `ok` at the barrier that
+    // each block and each item has anyway.
+    for (int r = 0; ok && next_item(p, r, it); ++r) {
       const int head = it.h0 + (p.pair_heads ? j : 0);
       const int r0 = it.r0 + (p.pair_heads ? 0 : j * BQ);
       const int rel = r0 + row;  // this thread's query, counted from the prompt's first token
       const int lo = p.window > 0 ? rel - p.window + 1 : 0;
-      float m = -INFINITY, l = 0.f;
-      for (int kb = it.kb0; ok && kb < it.kb1; ++kb, ++ns) {
-        ok = wait(&s_full[j], ns & 1);
-        if (!ok) break;
-        uint32_t s[4][32];
+      float m = -INFINITY, l = 0.f;  // the reference, in log2 units; the weights' sum over this thread's keys
+      for (int kb = it.kb0; kb < it.kb1; ++kb, ++ns) {
+        ok = wait(&s_full[j], ns & 1) && ok;
+        // The scores are read 16 columns at a time with the next 16 under way: all 64 would not fit the 96 registers
+        // that 18 warps leave a thread, and with this much shared memory a spill goes to L2.
+        const int k0 = kb * BKV + h * 64;
+        const bool cut = kb * BKV + BKV - 1 > r0 || (p.window > 0 && kb * BKV < r0 + BQ - p.window);
+        uint32_t s[2][16];
+        auto next_chunk = [&](int c, bool more) {
+          snb::tmem_ld_wait();
+          if (more) tmem_ld_x16(s_at + ((c + 1) & 3) * 16, s[(c + 1) & 1]);
+          if (cut) {
+            const int hi = rel - k0 - c * 16, from = lo - k0 - c * 16;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) snb::tmem_ld_32x32b_x32(s_at + c * 32, s[c]);
-        snb::tmem_ld_wait();
-        const int k0 = kb * BKV;
-        if (k0 + BKV - 1 > r0 || (p.window > 0 && k0 < r0 + BQ - p.window)) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const int key = k0 + c * 32 + i;
-              if (key > rel || key < lo) s[c][i] = 0xff800000u;
-            }
-        }
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) mx[c] = fmaxf(mx[c], __uint_as_float(s[c][i]));
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-        // The reference follows the maximum only when that has risen by more than 2^8: weights stay below 2^8, and
-        // the output in tensor memory is rarely read and written for it.
-        if (__any_sync(0xffffffffu, (top - m) * p.scale > 8.f || (m == -INFINITY && top > m))) {
-          const float mn = fmaxf(m, top);
-          const float f = mn == -INFINITY ? 1.f : ex2((m - mn) * p.scale);
-          l *= f;
-          m = mn;
-          if (kb > it.kb0) {
-            ok = wait(&o_full[j], (ns - 1) & 1);
-            if (!ok) break;
+            for (int i = 0; i < 16; ++i)
+              if (i > hi || i < from) s[c & 1][i] = 0xff800000u;
+          }
+        };
+        // The output in tensor memory follows a change of the reference by 2^-d, after the product `phase`.
+        auto rescale = [&](float f, int phase) {
+          ok = wait(&o_full[j], phase & 1);
 #pragma unroll 1
-            for (int c = 0; c < DV / 32; ++c) {
-              uint32_t o[32];
-              snb::tmem_ld_32x32b_x32(o_at + c * 32, o);
-              snb::tmem_ld_wait();
+          for (int c = 0; c < DV / 64; ++c) {
+            uint32_t o[32];
+            snb::tmem_ld_32x32b_x32(o_at + c * 32, o);
+            snb::tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-              tmem_st_x32(o_at + c * 32, o);
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+            tmem_st_x32(o_at + c * 32, o);
+          }
+        };
+        tmem_ld_x16(s_at, s[0]);
+        // Before the exponentials: the first block that a row sees sets its reference to that block's maximum. fp16
+        // weights have to stay below 2^16, so there every block's maximum is looked at, and the reference follows once
+        // it has risen by 2^8. (A row's two threads hold the same m: they agree on this branch.)
+        if (NARROW || __any_sync(0xffffffffu, m == -INFINITY)) {
+          float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            next_chunk(c, true);
+#pragma unroll
+            for (int i = 0; i < 16; i += 2)
+              mx[i / 2 & 1] = max3(mx[i / 2 & 1], __uint_as_float(s[c & 1][i]), __uint_as_float(s[c & 1][i + 1]));
+          }
+          const float top = fmaxf(mx[0], mx[1]) * p.scale;
+          const bool rise = m == -INFINITY ? top > m : top - m > 8.f;
+          if (bar_or(bar, rise || !ok)) {
+            if (bar_or(bar, !ok)) {
+              ok = false;
+              break;
             }
+            const float mn = fmaxf(m, exchange(top, [](float a, float b) { return fmaxf(a, b); }));
+            const float f = mn == -INFINITY ? 1.f : ex2(m - mn);
+            l *= f;
+            m = mn;
+            if (kb > it.kb0) rescale(f, ns - 1);
           }
         }
-        const float ref = m == -INFINITY ? 0.f : m * p.scale;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        const float ref = m == -INFINITY ? 0.f : -m;
+        const uint64_t scale2 = pair(p.scale, p.scale), ref2 = pair(ref, ref);
+        uint64_t sum[2] = {0, 0};
 #pragma unroll
-        for (int c = 0; c < 4; c += 2) {
-          uint32_t w2[32];
+        for (int c = 0; c < 4; ++c) {
+          uint32_t w2[8];
+          next_chunk(c, c < 3);
 #pragma unroll
-          for (int d = 0; d < 2; ++d)
-#pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              const float a = ex2(fmaf(__uint_as_float(s[c + d][i]), p.scale, -ref));
-              const float b = ex2(fmaf(__uint_as_float(s[c + d][i + 1]), p.scale, -ref));
-              sum[2 * d] += a;
-              sum[2 * d + 1] += b;
-              w2[d * 16 + i / 2] = pack2<T>(a, b);
+          for (int i = 0; i < 8; ++i) {
+            const uint64_t y = fma2(pair(__uint_as_float(s[c & 1][2 * i]), __uint_as_float(s[c & 1][2 * i + 1])), scale2,
+                                    ref2);
+            float2 e;
+            if (i % EMULATE == EMULATE - 1) {
+              e = exp2_fma<!NARROW>(y);
+            } else {
+              e = split(y);
+              e.x = ex2(e.x);
+              e.y = ex2(e.y);
             }
-          tmem_st_x32(s_at + c * 16, w2);
+            sum[i & 1] = add2(sum[i & 1], pair(e.x, e.y));
+            w2[i] = pack2<T>(e.x, e.y);
+          }
+          tmem_st_x8(s_at + c * 8, w2);
+          if (c & 1) {  // half of the weights: their product can start
+            tmem_st_wait();
+            snb::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) snb::mbar_arrive(&p_full[2 * j + c / 2]);
+          }
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        tmem_st_wait();
-        snb::tc_fence_before();
-        snb::mbar_arrive(&p_full[j]);
+        const float2 total = split(add2(sum[0], sum[1]));
+        const float block = total.x + total.y;
+        l += block;
+        // After them, off the critical path: bf16 weights have fp32's range, so a reference that lags costs no
+        // precision. It follows when a block's weights have come to more than 2^16; a weight past 2^128 in one step
+        // turns the row's output into an infinity, and such rows are computed once more below.
+        if (!NARROW && bar_or(bar, block > 65536.f || !ok)) {
+          if (bar_or(bar, !ok)) {
+            ok = false;
+            break;
+          }
+          const float most = exchange(block, [](float a, float b) { return fmaxf(a, b); });
+          const float up = most > 65536.f ? (float)((__float_as_int(most) >> 23) - 126) : 0.f;
+          const float f = ex2(-up);
+          l *= f;
+          m += up;
+          rescale(f, ns);
+        }
       }
       if (!ok) break;
       ok = wait(&o_full[j], (ns - 1) & 1);
-      if (!ok) break;
-      if (p.sinks != nullptr) l += ex2(p.sinks[head] * LOG2E - (m == -INFINITY ? 0.f : m * p.scale));
-      const float r = l > 0.f || l != l ? 1.f / l : 0.f;
+      if (bar_or(bar, !ok)) {
+        ok = false;
+        break;
+      }
+      l = exchange(l, [](float a, float b) { return a + b; });
+      if (p.sinks != nullptr) l += ex2(p.sinks[head] * LOG2E - (m == -INFINITY ? 0.f : m));
+      const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
       const bool store = rel < it.len;
       const int t = it.first + rel;
-      T* dst = reinterpret_cast<T*>(p.out) + (int64_t)t * p.os + (int64_t)head * DV;
+      T* dst = reinterpret_cast<T*>(p.out) + (int64_t)t * p.os + (int64_t)head * DV + h * (DV / 2);
       bool odd = false;
 #pragma unroll
-      for (int c = 0; c < DV / 32; ++c) {
+      for (int c = 0; c < DV / 64; ++c) {
         uint32_t o[32];
         snb::tmem_ld_32x32b_x32(o_at + c * 32, o);
         snb::tmem_ld_wait();
         uint32_t w2[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const float a = __uint_as_float(o[2 * i]) * r, b = __uint_as_float(o[2 * i + 1]) * r;
+          const float a = __uint_as_float(o[2 * i]) * inv, b = __uint_as_float(o[2 * i + 1]) * inv;
           odd |= !(fabsf(a) < INFINITY) || !(fabsf(b) < INFINITY);
           w2[i] = pack2<T>(a, b);
         }
@@ -489,17 +673,20 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       // A NaN or infinity in a masked value still meets a weight of 0 in the product (0 * inf = NaN): rows that came
       // out so are computed once more without touching what is masked.
-      unsigned again = __ballot_sync(0xffffffffu, odd && store);
-      while (again) {
-        const int src = __ffs(again) - 1;
-        again &= again - 1;
-        attend_row<T, D, DV>(p, it.first, it.first + r0 + (warp & 3) * 32 + src, head);
+      if (bar_or(bar, odd && store)) {
+        const bool either = exchange(odd && store ? 1.f : 0.f, [](float a, float b) { return fmaxf(a, b); }) > 0.f;
+        unsigned again = h == 0 ? __ballot_sync(0xffffffffu, either) : 0u;
+        while (again) {
+          const int src = __ffs(again) - 1;
+          again &= again - 1;
+          attend_row<T, D, DV>(p, it.first, it.first + r0 + (warp & 3) * 32 + src, head);
+        }
       }
     }
   }
   snb::tc_fence_before();
   __syncthreads();
-  if (warp == 8 && lane == 0) {
+  if (warp == LOAD_WARP && lane == 0) {
     // a CTA that stopped early still waits (bounded) for the loads it issued
     if (taken[0] < issued[0]) snb::mbar_wait_bounded(q_full, taken[0] & 1, status, SNB_ERR_TIMEOUT_TMA);
     for (int i = taken[1]; i < issued[1]; ++i)
@@ -507,7 +694,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     for (int i = taken[2]; i < issued[2]; ++i)
       if (!snb::mbar_wait_bounded(&v_full[i % C::NV], (i / C::NV) & 1, status, SNB_ERR_TIMEOUT_TMA)) break;
   }
-  if (warp == 9) snb::tmem_dealloc(tmem, 512);
+  if (warp == MMA_WARP) snb::tmem_dealloc(tmem, 512);
 }
 
 template <typename T, int D, int DV>
