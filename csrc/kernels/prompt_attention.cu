@@ -110,6 +110,9 @@ SNB_DEVICE float2 exp2_fma(uint64_t x) {
                      __int_as_float(__float_as_int(r.y) + (__float_as_int(ny.y) << 23)));
 }
 
+// Bits 0 .. n (none for n < 0, all for n > 31)
+SNB_DEVICE uint32_t upto(int n) { return n < 0 ? 0u : 0xffffffffu >> (31 - min(n, 31)); }
+
 struct PromptParams {
   const void *q, *k, *v;
   void* out;
@@ -119,6 +122,7 @@ struct PromptParams {
   int T, B, heads, kv_heads, window;
   float scale;  // of the scores, in log2 units
   int pair_heads, pairs, items;
+  int wide_out;  // output rows lie on 32-byte boundaries
   uint32_t idesc;  // the operands' type, for the MMA
 };
 
@@ -199,7 +203,7 @@ template <int D, int DV>
 struct Cfg {
   static constexpr int QB = D / 64 * CHUNK, KB = D / 64 * CHUNK, VB = DV / 64 * CHUNK;
   static constexpr int NK = D == 64 ? 4 : D == 128 ? 3 : 2, NV = D == 64 ? 4 : D == 128 ? 2 : 1;
-  static constexpr int SMEM = 2 * QB + NK * KB + NV * VB + 2 * BQ * 4 + 1024 + 512;
+  static constexpr int SMEM = 2 * QB + NK * KB + NV * VB + 2 * BQ * 4 + 1024 + 512;  // + exchange, alignment, barriers and items
 };
 
 // One lane of a converged warp; the compiler keeps what such a branch uses in uniform registers, which the MMA's
@@ -259,6 +263,12 @@ SNB_DEVICE bool bar_or(int id, bool v) {
       : "memory");
   return r != 0;
 }
+// 32 bytes, a whole sector: a row belongs to a thread, so a warp's store touches 32 rows
+SNB_DEVICE void st_global_v8(void* at, const uint32_t* r) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
 SNB_DEVICE void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // B operand whose rows (keys) are the contraction: 64-wide column chunks `CHUNK` bytes apart, 8-row groups 1024 apart
@@ -273,7 +283,7 @@ struct Item {
   int first, len;  // the prompt's first token and length
   int r0;          // first query row, counted from `first`
   int h0;          // head of the first tile
-  int kb0, kb1;    // key blocks [kb0, kb1), counted from `first`
+  int kb0, kb1;    // key blocks [kb0, kb1), counted from `first`; none: the list has ended
 };
 
 // Item w of the list (tile, head pair): the prompts in order, each prompt's tiles from its last one down. Called by
@@ -341,11 +351,14 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint64_t* s_full = v_empty + C::NV;  // [2] scores of a tile are in tensor memory
   uint64_t* p_full = s_full + 2;       // [2][2] the first / second half of a tile's weights are (its output rescaled)
   uint64_t* o_full = p_full + 4;       // [2] a tile's output has taken up a block
-  uint64_t* drain = o_full + 2;
+  uint64_t* i_full = o_full + 2;       // [2] a work item is in its slot
+  uint64_t* i_empty = i_full + 2;      // [2] and has been read by the softmax warps and the MMA warp
+  uint64_t* drain = i_empty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   int* issued = reinterpret_cast<int*>(tmem_slot + 1);  // loads issued: q, k, v
   int* taken = issued + 3;                              // and waited for
   float* sX = reinterpret_cast<float*>(taken + 3);      // [2][128] what the two halves of a row exchange
+  Item* sItem = reinterpret_cast<Item*>(sX + 2 * BQ);   // [2]
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -359,6 +372,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       snb::mbar_init(&p_full[2 * j + 1], 8);
       snb::mbar_init(&o_full[j], 1);
     }
+    for (int i = 0; i < 2; ++i) snb::mbar_init(&i_full[i], 1), snb::mbar_init(&i_empty[i], 17);
     snb::mbar_init(drain, 1);
     for (int i = 0; i < 6; ++i) issued[i] = 0;
     snb::fence_mbar_init();
@@ -378,9 +392,20 @@ __global__ void __launch_bounds__(THREADS, 1)
   if (warp == LOAD_WARP) {
     int nq = 0, nk = 0, nv = 0;
     bool ok = true;
-    Item it;
-    for (int r = 0; ok && next_item(p, r, it); ++r) {
+    // It alone works the items out (a few global reads and divisions), ahead of the warps that it hands them to.
+    for (int r = 0; ok; ++r) {
+      Item it;
+      const bool have = next_item(p, r, it);
+      if (!have) it.kb0 = it.kb1 = 0;
       if (lane == 0) {
+        ok = snb::mbar_wait_bounded(&i_empty[r & 1], ((r >> 1) & 1) ^ 1, status, SNB_ERR_TIMEOUT_TMA);
+        if (ok) {
+          sItem[r & 1] = it;
+          snb::mbar_arrive(&i_full[r & 1]);
+        }
+      }
+      if (!have) break;
+      if (lane == 0 && ok) {
         const int hk = it.h0 / G;
         auto load_k = [&](int kb) {
           const int s = nk % C::NK;
@@ -421,7 +446,6 @@ __global__ void __launch_bounds__(THREADS, 1)
   } else if (warp == MMA_WARP) {
     int nq = 0, nk = 0, nv = 0, np = 0;
     bool ok = true;
-    Item it;
     const uint32_t id_s = p.idesc | snb::idesc_bf16_f32(BQ, BKV) & ~(7u << 7 | 7u << 10);
     const uint32_t id_o = p.idesc | snb::idesc_bf16_f32(BQ, DV) & ~(7u << 7 | 7u << 10) | 1u << 16;
     const uint64_t q_desc = snb::smem_desc_sw128(snb::smem_u32(sQ)), k_desc = snb::smem_desc_sw128(snb::smem_u32(sK)),
@@ -459,8 +483,13 @@ __global__ void __launch_bounds__(THREADS, 1)
     auto commit = [&](uint64_t* bar) {
       if (elect_one()) snb::mma_commit(bar);
     };
-    for (int r = 0; ok && next_item(p, r, it); ++r) {
-      const int nb = it.kb1 - it.kb0;
+    for (int r = 0; ok; ++r) {
+      ok = wait(&i_full[r & 1], (r >> 1) & 1);
+      if (!ok) break;
+      const int nb = sItem[r & 1].kb1 - sItem[r & 1].kb0;
+      __syncwarp();
+      if (lane == 0) snb::mbar_arrive(&i_empty[r & 1]);
+      if (nb == 0) break;
       ok = wait(q_full, nq & 1) && wait(&k_full[nk % C::NK], (nk / C::NK) & 1);
       if (ok) {
         scores(0, nk % C::NK);
@@ -511,7 +540,6 @@ __global__ void __launch_bounds__(THREADS, 1)
     float* x = sX + j * BQ + row;
     int ns = 0;  // blocks done by this tile, over all items
     bool ok = true;
-    Item it;
     constexpr bool NARROW = std::is_same<T, __half>::value;
     auto wait = [&](uint64_t* b, int parity) {
       const bool r = snb::mbar_wait_bounded(b, parity, status, SNB_ERR_TIMEOUT_EPI);
@@ -528,10 +556,20 @@ __global__ void __launch_bounds__(THREADS, 1)
     };
     // A wait that ran out must end both warps of a pair at the same place: the pair agrees on `ok` at the barrier that
     // each block and each item has anyway.
-    for (int r = 0; ok && next_item(p, r, it); ++r) {
+    for (int r = 0; ok; ++r) {
+      ok = wait(&i_full[r & 1], (r >> 1) & 1);
+      if (bar_or(bar, !ok)) {
+        ok = false;
+        break;
+      }
+      const Item it = sItem[r & 1];
+      __syncwarp();
+      if (lane == 0) snb::mbar_arrive(&i_empty[r & 1]);
+      if (it.kb0 == it.kb1) break;
       const int head = it.h0 + (p.pair_heads ? j : 0);
       const int r0 = it.r0 + (p.pair_heads ? 0 : j * BQ);
       const int rel = r0 + row;  // this thread's query, counted from the prompt's first token
+      const int rw = r0 + (warp & 3) * 32;  // this warp's first query
       const int lo = p.window > 0 ? rel - p.window + 1 : 0;
       float m = -INFINITY, l = 0.f;  // the reference, in log2 units; the weights' sum over this thread's keys
       for (int kb = it.kb0; kb < it.kb1; ++kb, ++ns) {
@@ -539,16 +577,21 @@ __global__ void __launch_bounds__(THREADS, 1)
         // The scores are read 16 columns at a time with the next 16 under way: all 64 would not fit the 96 registers
         // that 18 warps leave a thread, and with this much shared memory a spill goes to L2.
         const int k0 = kb * BKV + h * 64;
-        const bool cut = kb * BKV + BKV - 1 > r0 || (p.window > 0 && kb * BKV < r0 + BQ - p.window);
         uint32_t s[2][16];
-        auto next_chunk = [&](int c, bool more) {
+        // What this warp's 32 rows see of 16 keys: nothing (0), a part (1) or all of them (2)
+        auto sight = [&](int c) {
+          const int kc = k0 + c * 16;
+          if (kc > rw + 31 || (p.window > 0 && kc + 15 <= rw - p.window)) return 0;
+          return kc + 15 > rw || (p.window > 0 && kc <= rw + 31 - p.window) ? 1 : 2;
+        };
+        auto next_chunk = [&](auto cut, int c, bool more) {
           snb::tmem_ld_wait();
           if (more) tmem_ld_x16(s_at + ((c + 1) & 3) * 16, s[(c + 1) & 1]);
-          if (cut) {
-            const int hi = rel - k0 - c * 16, from = lo - k0 - c * 16;
+          if (cut.value && sight(c) < 2) {
+            const uint32_t seen = upto(rel - k0 - c * 16) & ~upto(lo - 1 - k0 - c * 16);
 #pragma unroll
             for (int i = 0; i < 16; ++i)
-              if (i > hi || i < from) s[c & 1][i] = 0xff800000u;
+              if (!(seen >> i & 1)) s[c & 1][i] = 0xff800000u;
           }
         };
         // The output in tensor memory follows a change of the reference by 2^-d, after the product `phase`.
@@ -564,19 +607,27 @@ __global__ void __launch_bounds__(THREADS, 1)
             tmem_st_x32(o_at + c * 32, o);
           }
         };
+        // Blocks that every row sees whole take a path without the tests: those cost as much as the exponentials.
+        const bool ragged = kb * BKV + BKV - 1 > r0 || (p.window > 0 && kb * BKV < r0 + BQ - p.window);
         tmem_ld_x16(s_at, s[0]);
-        // Before the exponentials: the first block that a row sees sets its reference to that block's maximum. fp16
-        // weights have to stay below 2^16, so there every block's maximum is looked at, and the reference follows once
-        // it has risen by 2^8. (A row's two threads hold the same m: they agree on this branch.)
+        // Before the exponentials: a row's first block sets its reference to that block's maximum. For bf16 that may
+        // be the maximum of masked scores too: a reference far above what the row sees costs no precision, only range,
+        // and a row that runs out of it is computed once more below. fp16 weights have to lie between 2^-14 and 2^16,
+        // so there every block's maximum over what the row sees is looked at, and the reference follows once it has
+        // risen by 2^8. (A row's two threads hold the same m: they agree on this branch.)
         if (NARROW || __any_sync(0xffffffffu, m == -INFINITY)) {
           float mx[2] = {-INFINITY, -INFINITY};
+          auto maximum = [&](auto cut) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            next_chunk(c, true);
+            for (int c = 0; c < 4; ++c) {
+              next_chunk(cut, c, true);
 #pragma unroll
-            for (int i = 0; i < 16; i += 2)
-              mx[i / 2 & 1] = max3(mx[i / 2 & 1], __uint_as_float(s[c & 1][i]), __uint_as_float(s[c & 1][i + 1]));
-          }
+              for (int i = 0; i < 16; i += 2)
+                mx[i / 2 & 1] = max3(mx[i / 2 & 1], __uint_as_float(s[c & 1][i]), __uint_as_float(s[c & 1][i + 1]));
+            }
+          };
+          if (NARROW && ragged) maximum(std::true_type());
+          else maximum(std::false_type());
           const float top = fmaxf(mx[0], mx[1]) * p.scale;
           const bool rise = m == -INFINITY ? top > m : top - m > 8.f;
           if (bar_or(bar, rise || !ok)) {
@@ -594,33 +645,42 @@ __global__ void __launch_bounds__(THREADS, 1)
         const float ref = m == -INFINITY ? 0.f : -m;
         const uint64_t scale2 = pair(p.scale, p.scale), ref2 = pair(ref, ref);
         uint64_t sum[2] = {0, 0};
+        auto weights = [&](auto cut) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t w2[8];
-          next_chunk(c, c < 3);
+          for (int c = 0; c < 4; ++c) {
+            uint32_t w2[8];
+            next_chunk(cut, c, c < 3);
+            if (cut.value && sight(c) == 0) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const uint64_t y = fma2(pair(__uint_as_float(s[c & 1][2 * i]), __uint_as_float(s[c & 1][2 * i + 1])), scale2,
-                                    ref2);
-            float2 e;
-            if (i % EMULATE == EMULATE - 1) {
-              e = exp2_fma<!NARROW>(y);
+              for (int i = 0; i < 8; ++i) w2[i] = 0;
             } else {
-              e = split(y);
-              e.x = ex2(e.x);
-              e.y = ex2(e.y);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const uint64_t y = fma2(pair(__uint_as_float(s[c & 1][2 * i]), __uint_as_float(s[c & 1][2 * i + 1])),
+                                        scale2, ref2);
+                float2 e;
+                if (i % EMULATE == EMULATE - 1) {
+                  e = exp2_fma<!NARROW>(y);
+                } else {
+                  e = split(y);
+                  e.x = ex2(e.x);
+                  e.y = ex2(e.y);
+                }
+                sum[i & 1] = add2(sum[i & 1], pair(e.x, e.y));
+                w2[i] = pack2<T>(e.x, e.y);
+              }
             }
-            sum[i & 1] = add2(sum[i & 1], pair(e.x, e.y));
-            w2[i] = pack2<T>(e.x, e.y);
+            tmem_st_x8(s_at + c * 8, w2);
+            if (c & 1) {  // half of the weights: their product can start
+              tmem_st_wait();
+              snb::tc_fence_before();
+              __syncwarp();
+              if (lane == 0) snb::mbar_arrive(&p_full[2 * j + c / 2]);
+            }
           }
-          tmem_st_x8(s_at + c * 8, w2);
-          if (c & 1) {  // half of the weights: their product can start
-            tmem_st_wait();
-            snb::tc_fence_before();
-            __syncwarp();
-            if (lane == 0) snb::mbar_arrive(&p_full[2 * j + c / 2]);
-          }
-        }
+        };
+        if (ragged) weights(std::true_type());
+        else weights(std::false_type());
         const float2 total = split(add2(sum[0], sum[1]));
         const float block = total.x + total.y;
         l += block;
@@ -647,12 +707,13 @@ __global__ void __launch_bounds__(THREADS, 1)
         break;
       }
       l = exchange(l, [](float a, float b) { return a + b; });
+      // NaN if the sum over the keys left its range or an output is not finite
+      float zero = l > 0x1p-100f && l < 0x1p100f ? 0.f : NAN;
       if (p.sinks != nullptr) l += ex2(p.sinks[head] * LOG2E - (m == -INFINITY ? 0.f : m));
-      const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+      const float inv = m == -INFINITY ? 0.f : 1.f / l;  // only scores of -inf: nothing but the sink has weight
       const bool store = rel < it.len;
       const int t = it.first + rel;
       T* dst = reinterpret_cast<T*>(p.out) + (int64_t)t * p.os + (int64_t)head * DV + h * (DV / 2);
-      bool odd = false;
 #pragma unroll
       for (int c = 0; c < DV / 64; ++c) {
         uint32_t o[32];
@@ -662,17 +723,26 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const float a = __uint_as_float(o[2 * i]) * inv, b = __uint_as_float(o[2 * i + 1]) * inv;
-          odd |= !(fabsf(a) < INFINITY) || !(fabsf(b) < INFINITY);
+          zero = fmaf(a, 0.f, zero);
+          zero = fmaf(b, 0.f, zero);
           w2[i] = pack2<T>(a, b);
         }
-        if (store)
+        if (store) {
+          if (p.wide_out) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            *reinterpret_cast<uint4*>(dst + c * 32 + i * 8) =
-                make_uint4(w2[4 * i], w2[4 * i + 1], w2[4 * i + 2], w2[4 * i + 3]);
+            for (int i = 0; i < 2; ++i) st_global_v8(dst + c * 32 + i * 16, w2 + i * 8);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              *reinterpret_cast<uint4*>(dst + c * 32 + i * 8) =
+                  make_uint4(w2[4 * i], w2[4 * i + 1], w2[4 * i + 2], w2[4 * i + 3]);
+          }
+        }
       }
-      // A NaN or infinity in a masked value still meets a weight of 0 in the product (0 * inf = NaN): rows that came
-      // out so are computed once more without touching what is masked.
+      const bool odd = zero != 0.f;
+      // A NaN or infinity in a masked value still meets a weight of 0 in the product (0 * inf = NaN), and a masked
+      // score can have set the reference: rows that came out without a finite result are computed once more,
+      // touching nothing that is masked.
       if (bar_or(bar, odd && store)) {
         const bool either = exchange(odd && store ? 1.f : 0.f, [](float a, float b) { return fmaxf(a, b); }) > 0.f;
         unsigned again = h == 0 ? __ballot_sync(0xffffffffu, either) : 0u;
@@ -710,6 +780,7 @@ void launch(PromptParams p, int* status, cudaStream_t st) {
   p.idesc = bf16 ? 1u << 7 | 1u << 10 : 0u;
   p.pair_heads = (p.heads / p.kv_heads) % 2 == 0;
   p.pairs = p.pair_heads ? p.heads / 2 : p.heads;
+  p.wide_out = reinterpret_cast<uintptr_t>(p.out) % 32 == 0 && p.os % 16 == 0;
   const int rows = p.pair_heads ? BQ : 2 * BQ;
   const int64_t items = ((int64_t)p.T / rows + std::min(p.B, p.T)) * p.pairs;  // at most one ragged tile per prompt
   TORCH_CHECK(items < (int64_t(1) << 31), "prompt_attention: too much work for one call");

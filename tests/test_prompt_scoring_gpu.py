@@ -448,3 +448,31 @@ def test_operators_agree():
     b = token_logprobs(h.float() @ w.float().t(), ids)
     for x, y in zip(a[:3], b[:3]):
         assert _near(x, y, 1e-3)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_prompt_attention_masked_scores_tower_over_seen_ones(dtype):
+    """Keys that a row does not see score far above those that it sees: later tokens, and tokens behind the window."""
+    from sglang_neuron_b200.ops.prompt import prompt_attention
+    n, Hq, Hkv, D = 300, 2, 1, 64
+    _, _, v = _qkv(n, Hq, Hkv, D, D, dtype, seed=21)
+    q = torch.ones(n, Hq * D, device=DEV, dtype=dtype)
+    for step, window in ((0.5, 0), (-0.5, 20), (4.0, 0), (-4.0, 7)):
+        k = (torch.arange(n, device=DEV).float()[:, None] * step).expand(n, D).to(dtype).contiguous()
+        out = prompt_attention(q, k, v, _indptr([n]), Hq, Hkv, D, window=window)
+        _check_attention(out, q, k, v, [n], Hq, Hkv, D, D, window=window)
+
+
+def test_prompt_attention_all_scores_minus_infinity():
+    """Rows whose every score is -inf give zero, as the paged operators do; with a sink too."""
+    from sglang_neuron_b200.ops.prompt import prompt_attention
+    n, Hq, Hkv, D = 140, 2, 1, 64
+    q, k, v = (x.clone() for x in _qkv(n, Hq, Hkv, D, D, torch.bfloat16, seed=22))
+    q = q.abs() + 0.1
+    k[:50] = -math.inf
+    for sinks in (None, torch.zeros(Hq, device=DEV)):
+        out = prompt_attention(q, k, v, _indptr([n]), Hq, Hkv, D, sinks=sinks)
+        assert bool((out[:50] == 0).all()) and bool(torch.isfinite(out.float()).all())
+        seen = prompt_attention(q[50:], k[50:], v[50:], _indptr([n - 50]), Hq, Hkv, D, sinks=sinks)
+        tol = (4 * U[torch.bfloat16] + 8e-4) * v.float().abs().max().item()
+        assert ((out[50:].float() - seen.float()).abs() <= tol).all()
