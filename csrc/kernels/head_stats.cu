@@ -508,14 +508,13 @@ __global__ void __launch_bounds__(256)
 }
 
 void join_parts(const at::Tensor& part, const float* chosen, int pitch, int N, int V, int tiles, int width,
-                const int64_t* ids, int64_t vocab_offset, at::Tensor& logprobs, at::Tensor& entropy, at::Tensor& lse,
-                cudaStream_t st) {
+                const int64_t* ids, int64_t vocab_offset, at::Tensor& stats, cudaStream_t st) {
+  float* out = stats.data_ptr<float>();
   // one row per CTA until the CTAs would come in many waves
   const bool one = N <= 2048;
   C10_CUDA_CHECK(snb::launch_pdl(one ? head_join_kernel<1> : head_join_kernel<8>, dim3(one ? N : (N + 7) / 8),
                                  dim3(256), 0, st, reinterpret_cast<const float4*>(part.data_ptr<float>()), chosen,
-                                 pitch, N, V, tiles, width, ids, vocab_offset, logprobs.data_ptr<float>(),
-                                 entropy.data_ptr<float>(), lse.data_ptr<float>()));
+                                 pitch, N, V, tiles, width, ids, vocab_offset, out, out + N, out + 2 * N));
 }
 
 cudaLaunchConfig_t pair_config(cudaLaunchAttribute* attr) {
@@ -564,19 +563,20 @@ int pick_width(int mt, int64_t V, int pairs) {
 
 }  // namespace
 
-// hidden [N, K], weight [>= V, K] (or 128 x 64 tiles, `tiled`), both bf16 or both fp16; ids [N] int64; outputs [N].
-void head_stats(at::Tensor hidden, at::Tensor weight, int64_t V, bool tiled, at::Tensor ids,
-                int64_t vocab_offset, at::Tensor logprobs, at::Tensor entropy, at::Tensor lse,
-                at::Tensor status) {
+// hidden [N, K], weight [>= V, K] (or 128 x 64 tiles, `tiled`), both bf16 or both fp16; ids [N] int64. Returns fp32
+// [3, N]: log-probability, entropy, log-sum-exp.
+at::Tensor head_stats(at::Tensor hidden, at::Tensor weight, int64_t V, bool tiled, at::Tensor ids,
+                      int64_t vocab_offset, at::Tensor status) {
   const int64_t N = hidden.size(0), K = hidden.size(1);
   TORCH_CHECK(hidden.is_cuda() && hidden.stride(1) == 1 && weight.stride(1) == 1, "head_logprobs: row-major operands");
   TORCH_CHECK(hidden.scalar_type() == weight.scalar_type() &&
                   (hidden.scalar_type() == at::kBFloat16 || hidden.scalar_type() == at::kHalf),
               "head_logprobs: bf16 or fp16 operands of one type");
-  TORCH_CHECK(ids.scalar_type() == at::kLong && ids.is_contiguous() && ids.numel() == N,
+  TORCH_CHECK(ids.is_cuda() && ids.scalar_type() == at::kLong && ids.is_contiguous() && ids.numel() == N,
               "head_logprobs: one int64 id per row");
   TORCH_CHECK(K > 0 && V > 0 && V < (int64_t(1) << 30) && N < (int64_t(1) << 30), "head_logprobs: sizes");
-  if (N == 0) return;
+  auto stats = at::empty({3, N}, hidden.options().dtype(at::kFloat));
+  if (N == 0) return stats;
   const bool bf16 = hidden.scalar_type() == at::kBFloat16;
   const auto dt = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   auto st = at::cuda::getCurrentCUDAStream();
@@ -611,8 +611,8 @@ void head_stats(at::Tensor hidden, at::Tensor weight, int64_t V, bool tiled, at:
     const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
     C10_CUDA_CHECK(cudaFuncSetAttribute(head_few_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
     C10_CUDA_CHECK(snb::launch_pdl(head_few_kernel, dim3(std::min(groups, sms)), dim3(THREADS), SMEM, st, th, tw, tw32, p));
-    join_parts(part, p.chosen, (int)N, (int)N, (int)V, groups, GROUP, p.ids, vocab_offset, logprobs, entropy, lse, st);
-    return;
+    join_parts(part, p.chosen, (int)N, (int)N, (int)V, groups, GROUP, p.ids, vocab_offset, stats, st);
+    return stats;
   }
   const CUtensorMap th = snb_host::make_tmap_2d(hidden.data_ptr(), dt, K, N, hidden.stride(0) * 2, BK, BM,
                                                 CU_TENSOR_MAP_SWIZZLE_128B);
@@ -648,5 +648,6 @@ void head_stats(at::Tensor hidden, at::Tensor weight, int64_t V, bool tiled, at:
   cfg.stream = st;
   cfg.numAttrs = snb::pdl_enabled() ? 2 : 1;
   C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, head_stats_kernel, th, tw, p));
-  join_parts(part, nullptr, n_pad, (int)N, (int)V, vt, width, p.ids, vocab_offset, logprobs, entropy, lse, st);
+  join_parts(part, nullptr, n_pad, (int)N, (int)V, vt, width, p.ids, vocab_offset, stats, st);
+  return stats;
 }

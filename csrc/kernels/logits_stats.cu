@@ -7,34 +7,50 @@
 // the other way round.
 //
 // The best K entries (value descending, ties to the lower id) come from the same pass: a warp reads 512 contiguous
-// bytes per load (a segment) and keeps the segment's maximum, which the running reference needs anyway. The K-th
+// bytes per load and keeps the maximum of every two loads (a segment), which the running reference needs anyway. The K-th
 // best of the threads' maxima is a lower bound of the K-th best entry, so afterwards only the segments whose
 // maximum reaches it are read again (they are in L2) and sorted in by (value, ~id) keys: about K segments for
 // ordinary rows, all of them for a constant row.
 //
-// Bound: the logits' bytes at DRAM rate. Per logit the arithmetic is one exponential (16 a clock and SM, the
-// nearest limit: a bf16 row at full DRAM rate asks for about 12) and six simple instructions.
-// Split: one CTA of 256 threads per row, four resident per SM; fewer rows than that put a cluster of 2 to 8 CTAs
-// on each row, whose partial results the first CTA joins through distributed shared memory.
+// Bound: the logits' bytes at DRAM rate. A bf16 row at that rate brings 12 logits a clock and SM, so a logit has one
+// exponential (of 16 a clock) and few issue slots: two values go through each fp32 instruction (f32x2), y is taken in
+// units of log 2 by one multiply-add, maximum and floor act on the 16-bit pairs as loaded. The floor (-2^100, fp16
+// -6e4) keeps 0 * y finite where a logit is masked; a CTA whose every logit lies down there reads its part once more
+// on an exact path.
+// The row comes through a ring of three 16 KB bulk copies that one thread keeps full.
+// Split: one CTA per row, four resident per SM; fewer rows than that put a cluster of 2 to 8 CTAs on each row, whose
+// partial results the first CTA joins through distributed shared memory.
 #include <ATen/core/Tensor.h>
+#include <ATen/ops/empty.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAException.h>
 #include "../common.cuh"
 #include <algorithm>
+#include <tuple>
 
 namespace {
 
-constexpr int THREADS = 256;
-constexpr int WARPS = THREADS / 32;
-constexpr int UNROLL = 4;       // segments in flight per warp
+constexpr int WARPS = 8;        // that read the row; one more keeps the ring full
+constexpr int THREADS = (WARPS + 1) * 32;
+constexpr int STAGES = 3;
+constexpr int PER = 4;                    // segments that a warp reads of a stage
+constexpr int STAGE_UNITS = PER * WARPS;
+constexpr int STAGE_BYTES = STAGE_UNITS * 512;
+constexpr int AHEAD = 4;        // selected segments that a warp reads again at a time
 constexpr int MAX_TOP = 32;     // one entry per lane of a warp's sorted list
 constexpr int MAX_CLUSTER = 8;  // the portable cluster size
 constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LN2 = 0.6931471805599453f;
 
 // max that keeps a NaN
 SNB_DEVICE float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+SNB_DEVICE float warp_max_nan(float v) {
+  float r;
+  asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
   return r;
 }
 SNB_DEVICE float ex2(float x) {
@@ -53,37 +69,98 @@ SNB_DEVICE float key_value(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
+// two fp32 values in a 64-bit register pair
+SNB_DEVICE uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+SNB_DEVICE float2 split(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+SNB_DEVICE uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+SNB_DEVICE uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+SNB_DEVICE uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// A 16-byte vector of logits. maximum(): of all its values, a NaN stays one. floor(): with values below FLOOR (exact
+// in the type) raised to it; that changes nothing where the maximum is above LOWEST. two(): values 2 i and 2 i + 1.
 template <typename T>
 struct Vec;
 template <>
 struct Vec<float> {
   static constexpr int N = 4;
-  static SNB_DEVICE void unpack(const uint4& u, float (&f)[4]) {
-    f[0] = __uint_as_float(u.x);
-    f[1] = __uint_as_float(u.y);
-    f[2] = __uint_as_float(u.z);
-    f[3] = __uint_as_float(u.w);
+  static constexpr float FLOOR = -0x1p100f, LOWEST = -0x1p99f;
+  static constexpr uint32_t NONE = 0xff800000u;
+  static SNB_DEVICE float2 two(const uint4& u, int i) {
+    return i == 0 ? make_float2(__uint_as_float(u.x), __uint_as_float(u.y))
+                  : make_float2(__uint_as_float(u.z), __uint_as_float(u.w));
+  }
+  static SNB_DEVICE float maximum(const uint4& u) {
+    return max_nan(max_nan(__uint_as_float(u.x), __uint_as_float(u.y)),
+                   max_nan(__uint_as_float(u.z), __uint_as_float(u.w)));
+  }
+  static SNB_DEVICE uint4 floor(const uint4& u) {
+    return make_uint4(__float_as_uint(max_nan(__uint_as_float(u.x), FLOOR)),
+                      __float_as_uint(max_nan(__uint_as_float(u.y), FLOOR)),
+                      __float_as_uint(max_nan(__uint_as_float(u.z), FLOOR)),
+                      __float_as_uint(max_nan(__uint_as_float(u.w), FLOOR)));
   }
   static SNB_DEVICE float one(float v) { return v; }
 };
-template <>
-struct Vec<__nv_bfloat16> {
+// the 16-bit types: two values in a word
+template <typename T, typename T2>
+struct Vec16 {
   static constexpr int N = 8;
-  static SNB_DEVICE void unpack(const uint4& u, float (&f)[8]) { snb::unpack_bf16x8(u, f); }
+  static SNB_DEVICE uint32_t word(const uint4& u, int i) { return i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w; }
+  static SNB_DEVICE T2 as(uint32_t w) { return *reinterpret_cast<const T2*>(&w); }
+  static SNB_DEVICE uint32_t bits(T2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
+  static SNB_DEVICE T2 most(const uint4& u) {
+    return __hmax2_nan(__hmax2_nan(as(u.x), as(u.y)), __hmax2_nan(as(u.z), as(u.w)));
+  }
+  static SNB_DEVICE uint4 raise(const uint4& u, T2 f) {
+    return make_uint4(bits(__hmax2_nan(as(u.x), f)), bits(__hmax2_nan(as(u.y), f)), bits(__hmax2_nan(as(u.z), f)),
+                      bits(__hmax2_nan(as(u.w), f)));
+  }
+};
+template <>
+struct Vec<__nv_bfloat16> : Vec16<__nv_bfloat16, __nv_bfloat162> {
+  static constexpr float FLOOR = -0x1p100f, LOWEST = -0x1p99f;
+  static constexpr uint32_t NONE = 0xff80ff80u;
+  static SNB_DEVICE float2 two(const uint4& u, int i) {
+    const uint32_t w = word(u, i);
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  }
+  static SNB_DEVICE float maximum(const uint4& u) {
+    const uint32_t w = bits(most(u));
+    return max_nan(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  }
+  static SNB_DEVICE uint4 floor(const uint4& u) { return raise(u, __float2bfloat162_rn(FLOOR)); }
   static SNB_DEVICE float one(__nv_bfloat16 v) { return __bfloat162float(v); }
 };
 template <>
-struct Vec<__half> {
-  static constexpr int N = 8;
-  static SNB_DEVICE void unpack(const uint4& u, float (&f)[8]) {
-    const __half2* h = reinterpret_cast<const __half2*>(&u);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 t = __half22float2(h[i]);
-      f[2 * i] = t.x;
-      f[2 * i + 1] = t.y;
-    }
+struct Vec<__half> : Vec16<__half, __half2> {
+  static constexpr float FLOOR = -6e4f, LOWEST = -5.9e4f;
+  static constexpr uint32_t NONE = 0xfc00fc00u;
+  static SNB_DEVICE float2 two(const uint4& u, int i) { return __half22float2(as(word(u, i))); }
+  static SNB_DEVICE float maximum(const uint4& u) {
+    const float2 m = __half22float2(most(u));
+    return max_nan(m.x, m.y);
   }
+  static SNB_DEVICE uint4 floor(const uint4& u) { return raise(u, __float2half2_rn(FLOOR)); }
   static SNB_DEVICE float one(__half v) { return __half2float(v); }
 };
 
@@ -123,19 +200,31 @@ template <typename T, bool TOP>
 __global__ void __launch_bounds__(THREADS, 4)
     logits_stats_kernel(const T* __restrict__ logits, int64_t stride, int V, const int64_t* __restrict__ ids,
                         int64_t vocab_offset, int K, float* __restrict__ logprobs, float* __restrict__ entropy,
-                        float* __restrict__ lse_out, float* __restrict__ top_vals, int64_t* __restrict__ top_ids) {
+                        float* __restrict__ lse_out, float* __restrict__ top_vals, int64_t* __restrict__ top_ids,
+                        int* status) {
   constexpr int N = Vec<T>::N;
-  extern __shared__ uint32_t seg_key[];  // [units of this CTA + 1]: the segments' maxima, the ragged ends last
+  extern __shared__ __align__(128) uint8_t dyn[];  // the ring, then the segments' maxima
+  float* seg_max = reinterpret_cast<float*>(dyn + STAGES * STAGE_BYTES);
+  __shared__ uint64_t full[STAGES], empty[STAGES];
   __shared__ Stats warp_stats[WARPS];
+  __shared__ float warp_best[WARPS + 1];
   __shared__ Stats cta_stats[MAX_CLUSTER];
   __shared__ uint64_t cand[WARPS * MAX_TOP];
-  __shared__ uint64_t best[MAX_CLUSTER * MAX_TOP];  // filled by every CTA of the cluster in the first one's memory
+  __shared__ uint64_t lists[MAX_CLUSTER * MAX_TOP];  // filled by every CTA of the cluster in the first one's memory
   __shared__ int cand_n, best_n[MAX_CLUSTER];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int C = gridDim.x, rank = blockIdx.x;  // the cluster spans the grid's x axis
   const int64_t row = blockIdx.y;
-  if (TOP && threadIdx.x == 0) cand_n = 0;
+  if (threadIdx.x == 0) {
+    if (TOP) cand_n = 0;
+    for (int i = 0; i < STAGES; ++i) {
+      snb::mbar_init(&full[i], 1);
+      snb::mbar_init(&empty[i], WARPS);
+    }
+    snb::fence_mbar_init();
+  }
+  __syncthreads();
   snb::pdl_wait();
   snb::pdl_trigger();
   const T* x = logits + row * stride;
@@ -143,53 +232,82 @@ __global__ void __launch_bounds__(THREADS, 4)
   const uint4* body = reinterpret_cast<const uint4*>(x + cut.head);
   const int u0 = (int)((int64_t)rank * cut.units / C), u1 = (int)((int64_t)(rank + 1) * cut.units / C);
 
-  Stats st{-INFINITY, 0.f, 0.f};
-  uint32_t best_key = 0;
-  auto add = [&](const float* v, int n, float mx) {
-    // mx: the maximum of v[0..n); -inf: nothing to add
-    if (mx == -INFINITY) return;
-    if (!(mx <= st.c)) {  // also when mx is NaN
-      const float f = ex2((st.c - mx) * LOG2E);
-      st.t = f > 0.f ? f * (st.t + st.s * (st.c - mx)) : 0.f;
-      st.s *= f;
-      st.c = mx;
+  float cl = -INFINITY;  // the reference times log2 e; two partial sums each, in the halves of a pair
+  uint64_t s2 = 0, t2 = 0;
+  float best = -INFINITY;  // this thread's maximum
+  bool any = false;        // this thread has seen a logit
+  const uint64_t log2e2 = pair(LOG2E, LOG2E);
+  auto take = [&](const uint4& a, const uint4& b, float mx) {
+    const float ml = max_nan(mx, Vec<T>::FLOOR) * LOG2E;
+    if (ml > cl || ml != ml) {  // a reference that has become NaN stays one
+      const float f = ex2(cl - ml), d = cl - ml;
+      const uint64_t f2 = pair(f, f);
+      // sums that weigh nothing now must not meet an infinite distance
+      t2 = f > 0.f ? mul2(fma2(s2, pair(d, d), t2), f2) : 0;
+      s2 = mul2(s2, f2);
+      cl = ml;
     }
+    const uint64_t c2 = pair(-cl, -cl);
 #pragma unroll
-    for (int i = 0; i < n; ++i) {
-      // a logit of -inf has weight 0: the floor keeps 0 * y finite
-      const float y = max_nan(v[i] - st.c, -1e30f);
-      const float e = ex2(y * LOG2E);
-      st.s += e;
-      st.t = fmaf(e, y, st.t);
+    for (int h = 0; h < 2; ++h) {
+      const uint4 r = Vec<T>::floor(h == 0 ? a : b);
+#pragma unroll
+      for (int k = 0; k < N / 2; ++k) {
+        const float2 v = Vec<T>::two(r, k);
+        const uint64_t y2 = fma2(pair(v.x, v.y), log2e2, c2);
+        const float2 y = split(y2);
+        const uint64_t e2 = pair(ex2(y.x), ex2(y.y));
+        s2 = add2(s2, e2);
+        t2 = fma2(e2, y2, t2);
+      }
     }
   };
 
-  for (int u = u0 + warp; u < u1; u += WARPS * UNROLL) {
-    uint4 raw[UNROLL];
-#pragma unroll
-    for (int j = 0; j < UNROLL; ++j) {
-      const int uj = u + j * WARPS, iv = uj * 32 + lane;
-      if (uj < u1 && iv < cut.nvec) raw[j] = __ldg(body + iv);
+  const int v0 = u0 * 32, v1 = min(u1 * 32, cut.nvec);  // this CTA's vectors
+  const int stages = (u1 - u0 + STAGE_UNITS - 1) / STAGE_UNITS;
+  if (warp == WARPS) {
+    if (lane == 0) {
+      int i = 0;
+      for (; i < stages; ++i) {
+        const int b = i % STAGES;
+        if (!snb::mbar_wait_bounded(&empty[b], ((i / STAGES) & 1) ^ 1, status, SNB_ERR_TIMEOUT_TMA)) break;
+        const int v = v0 + i * STAGE_UNITS * 32;
+        const uint32_t bytes = min(STAGE_BYTES, (v1 - v) * 16);
+        snb::mbar_arrive_expect_tx(&full[b], bytes);
+        snb::bulk_load(dyn + b * STAGE_BYTES, body + v, bytes, &full[b]);
+      }
+      // nothing is in flight when the memory goes away, even if the readers gave up
+      for (int d = max(0, i - STAGES); d < i; ++d)
+        snb::mbar_wait_bounded(&full[d % STAGES], (d / STAGES) & 1, status, SNB_ERR_TIMEOUT_TMA);
     }
+    __syncwarp();
+  } else {
+    for (int i = 0; i < stages; ++i) {
+      const int b = i % STAGES;
+      const bool ok = snb::mbar_wait_bounded(&full[b], (i / STAGES) & 1, status, SNB_ERR_TIMEOUT_MMA);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      uint4 raw[PER];
+      const int first = u0 + i * STAGE_UNITS + warp;
 #pragma unroll
-    for (int j = 0; j < UNROLL; ++j) {
-      const int uj = u + j * WARPS;
-      if (uj >= u1) break;
-      float v[N], mx = -INFINITY;
-      const bool have = uj * 32 + lane < cut.nvec;
-      if (have) {
-        Vec<T>::unpack(raw[j], v);
-        mx = v[0];
+      for (int h = 0; h < PER; ++h) {
+        const int uj = first + h * WARPS;
+        const bool have = uj < u1 && uj * 32 + lane < cut.nvec;
+        raw[h] = make_uint4(Vec<T>::NONE, Vec<T>::NONE, Vec<T>::NONE, Vec<T>::NONE);  // all -inf: adds nothing
+        if (have) raw[h] = *reinterpret_cast<const uint4*>(dyn + b * STAGE_BYTES + ((h * WARPS + warp) * 32 + lane) * 16);
+        any |= have;
+      }
 #pragma unroll
-        for (int i = 1; i < N; ++i) mx = max_nan(mx, v[i]);
-        add(v, N, mx);
+      for (int h = 0; h < PER; h += 2) {
+        const float mx = max_nan(Vec<T>::maximum(raw[h]), Vec<T>::maximum(raw[h + 1]));
+        best = max_nan(best, mx);
+        take(raw[h], raw[h + 1], mx);
+        if constexpr (TOP) {
+          const float seg = warp_max_nan(mx);
+          if (lane == 0 && first + h * WARPS < u1) seg_max[((i * PER + h) / 2) * WARPS + warp] = seg;
+        }
       }
-      if constexpr (TOP) {
-        const uint32_t k = have ? order_key(mx) : 0u;
-        best_key = max(best_key, k);
-        const uint32_t seg = __reduce_max_sync(0xffffffffu, k);
-        if (lane == 0) seg_key[uj - u0] = seg;
-      }
+      __syncwarp();
+      if (lane == 0) snb::mbar_arrive(&empty[b]);
     }
   }
   // the ragged ends (head and tail, fewer than two vectors) belong to the first CTA's first warp
@@ -198,10 +316,53 @@ __global__ void __launch_bounds__(THREADS, 4)
   const int end_i = lane < cut.head ? lane : cut.tail0 + lane - cut.head;
   float end_v = -INFINITY;
   if (mine) {
+    any = true;
     end_v = Vec<T>::one(x[end_i]);
-    add(&end_v, 1, end_v);
-    if (TOP) best_key = max(best_key, order_key(end_v));
+    best = max_nan(best, end_v);
   }
+  {
+    const float m = warp_max_nan(best);
+    if (lane == 0) warp_best[warp] = m;
+  }
+  __syncthreads();
+  float most = warp_best[0];
+#pragma unroll
+  for (int i = 1; i <= WARPS; ++i) most = max_nan(most, warp_best[i]);
+
+  // to natural units, against the thread's own maximum: cl is its product with log2 e, rounded
+  Stats st{-INFINITY, 0.f, 0.f};
+  auto exact = [&](float v) {
+    if (v == -INFINITY) return;
+    if (v > st.c || v != v) {
+      const float f = ex2((st.c - v) * LOG2E);
+      st.t = f > 0.f ? f * (st.t + st.s * (st.c - v)) : 0.f;
+      st.s *= f;
+      st.c = v;
+    }
+    const float y = max_nan(v - st.c, -1e30f), e = ex2(y * LOG2E);
+    st.s += e;
+    st.t = fmaf(e, y, st.t);
+  };
+  if (most <= Vec<T>::LOWEST || most > 1e30f) {
+    if (warp < WARPS && most != -INFINITY)
+      for (int u = u0 + warp; u < u1; u += WARPS) {
+        if (u * 32 + lane >= cut.nvec) continue;
+        const uint4 raw = __ldg(body + u * 32 + lane);
+#pragma unroll 1
+        for (int k = 0; k < N / 2; ++k) {
+          const float2 v = Vec<T>::two(raw, k);
+          exact(v.x);
+          exact(v.y);
+        }
+      }
+  } else if (!(cl <= Vec<T>::FLOOR * LOG2E)) {
+    const float2 ss = split(s2), ts = split(t2);
+    st.c = cl * (1.f / LOG2E);
+    const float off = fmaf(-st.c, LOG2E, cl), f = ex2(off);
+    st.s = (ss.x + ss.y) * f;
+    st.t = ((ts.x + ts.y) + (ss.x + ss.y) * off) * f * LN2;
+  }
+  if (mine) exact(end_v);
 
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
@@ -212,21 +373,26 @@ __global__ void __launch_bounds__(THREADS, 4)
     // both lanes of a pair join in the same order: every lane ends with the same bits
     st = (lane & o) ? join(b, st) : join(st, b);
   }
-  if (lane == 0) warp_stats[warp] = st;
+  if (lane == 0 && warp < WARPS) warp_stats[warp] = st;
 
   if constexpr (TOP) {
-    // the K-th largest of the threads' maxima, bit by bit (0 when fewer than K threads hold any entry)
+    // a lower bound of the K-th best entry: the K-th largest of the threads' maxima, to the upper 16 bits of its key
+    // (0 when fewer than K threads hold any entry)
+    const uint32_t best_key = any ? order_key(best) : 0u;
     uint32_t thr = 0;
 #pragma unroll 1
-    for (int b = 31; b >= 0; --b) {
+    for (int b = 31; b >= 16; --b) {
       const uint32_t t = thr | (1u << b);
       if (__syncthreads_count(best_key >= t) >= K) thr = t;
     }
     // every warp sorts the entries >= thr of its own segments into a list held across its lanes
     uint64_t list = 0;
-    auto offer = [&](uint64_t key) {
+    auto offer = [&](bool have, float v, uint32_t i) {
+      const uint32_t k32 = order_key(v);
+      if (!__ballot_sync(0xffffffffu, have && k32 >= thr)) return;
+      const uint64_t key = have ? ((uint64_t)k32 << 32) | (0xffffffffu - i) : 0ull;
       const uint64_t kth = __shfl_sync(0xffffffffu, list, K - 1);
-      unsigned hit = __ballot_sync(0xffffffffu, key > kth && (uint32_t)(key >> 32) >= thr);
+      unsigned hit = __ballot_sync(0xffffffffu, key > kth && k32 >= thr);
       while (hit) {
         const int src = __ffs(hit) - 1;
         hit &= hit - 1;
@@ -235,25 +401,37 @@ __global__ void __launch_bounds__(THREADS, 4)
         if (k > list) list = (lane > 0 && k > up) ? up : k;
       }
     };
-    const int mine_n = u1 - u0 - warp > 0 ? (u1 - u0 - warp + WARPS - 1) / WARPS : 0;
+    const int mine_n = warp < WARPS && u1 - u0 - warp > 0 ? (u1 - u0 - warp + 2 * WARPS - 1) / (2 * WARPS) : 0;
 #pragma unroll 1
     for (int j0 = 0; j0 < mine_n; j0 += 32) {
       const int j = j0 + lane;
-      unsigned sel = __ballot_sync(0xffffffffu, j < mine_n && seg_key[warp + j * WARPS] >= thr);
+      unsigned sel = __ballot_sync(0xffffffffu, j < mine_n && order_key(seg_max[warp + j * WARPS]) >= thr);
       while (sel) {
-        const int uj = u0 + warp + (j0 + __ffs(sel) - 1) * WARPS;
-        sel &= sel - 1;
-        const int iv = uj * 32 + lane;
-        float v[N];
-        const bool have = iv < cut.nvec;
-        if (have) Vec<T>::unpack(__ldg(body + iv), v);
-        const uint32_t i0 = (uint32_t)(cut.head + iv * N);
+        uint4 raw[AHEAD];
+        int iv[AHEAD];
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-          offer(have ? ((uint64_t)order_key(v[i]) << 32) | (0xffffffffu - (i0 + i)) : 0ull);
+        for (int n = 0; n < AHEAD; ++n) {  // a segment is two of the warp's units
+          const int un = sel ? u0 + warp + (2 * (j0 + __ffs(sel) - 1) + n % 2) * WARPS : u1;
+          iv[n] = un < u1 ? un * 32 + lane : cut.nvec;
+          if (n % 2) sel &= sel - 1;
+          raw[n] = make_uint4(0, 0, 0, 0);
+          if (iv[n] < cut.nvec) raw[n] = __ldg(body + iv[n]);
+        }
+#pragma unroll
+        for (int n = 0; n < AHEAD; ++n) {
+          const bool have = iv[n] < cut.nvec;
+          if (!__any_sync(0xffffffffu, have)) continue;
+          const uint32_t i0 = (uint32_t)(cut.head + iv[n] * N);
+#pragma unroll
+          for (int i = 0; i < N / 2; ++i) {
+            const float2 v = Vec<T>::two(raw[n], i);
+            offer(have, v.x, i0 + 2 * i);
+            offer(have, v.y, i0 + 2 * i + 1);
+          }
+        }
       }
     }
-    if (warp == 0) offer(mine ? ((uint64_t)order_key(end_v) << 32) | (0xffffffffu - (uint32_t)end_i) : 0ull);
+    if (warp == 0) offer(mine, end_v, (uint32_t)end_i);
     const bool valid = lane < K && list != 0;
     const unsigned vm = __ballot_sync(0xffffffffu, valid);
     int base = 0;
@@ -283,13 +461,13 @@ __global__ void __launch_bounds__(THREADS, 4)
     }
   }
   if constexpr (TOP) {
-    const int n = cand_n;
+    const int n = cand_n;  // at most WARPS * MAX_TOP
     for (int i = threadIdx.x; i < n; i += THREADS) {
       const uint64_t k = cand[i];
       int r = 0;
       for (int j = 0; j < n; ++j) r += cand[j] > k;
       if (r < K) {
-        const uint32_t at = snb::mapa_shared(snb::smem_u32(&best[rank * MAX_TOP + r]), dst_rank);
+        const uint32_t at = snb::mapa_shared(snb::smem_u32(&lists[rank * MAX_TOP + r]), dst_rank);
         asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(at), "l"(k) : "memory");
       }
     }
@@ -324,11 +502,17 @@ __global__ void __launch_bounds__(THREADS, 4)
     for (int i = threadIdx.x; i < C * MAX_TOP; i += THREADS) {
       const int r = i / MAX_TOP, p = i % MAX_TOP;
       if (p >= best_n[r]) continue;
-      const uint64_t k = best[i];
+      const uint64_t k = lists[i];
       int at = p;  // the lists are sorted and their keys differ: the place in the merged list is the sum of ranks
       for (int q = 0; q < C; ++q) {
         if (q == r) continue;
-        for (int j = 0; j < best_n[q] && best[q * MAX_TOP + j] > k; ++j) ++at;
+        int lo = 0, hi = best_n[q];  // how many of list q come before
+        while (lo < hi) {
+          const int mid = (lo + hi) / 2;
+          if (lists[q * MAX_TOP + mid] > k) lo = mid + 1;
+          else hi = mid;
+        }
+        at += lo;
       }
       if (at < K) {
         top_vals[row * K + at] = none ? -INFINITY : (key_value((uint32_t)(k >> 32)) - a.c) - lg;
@@ -340,8 +524,7 @@ __global__ void __launch_bounds__(THREADS, 4)
 
 template <typename T>
 void launch(const at::Tensor& logits, int V, const at::Tensor& ids, int64_t vocab_offset, int K,
-            at::Tensor& logprobs, at::Tensor& entropy, at::Tensor& lse, at::Tensor& top_vals,
-            at::Tensor& top_ids) {
+            at::Tensor& stats, at::Tensor& top_vals, at::Tensor& top_ids, int* status) {
   const int64_t rows = logits.size(0);
   const auto* prop = at::cuda::getCurrentDeviceProperties();
   auto st = at::cuda::getCurrentCUDAStream();
@@ -349,7 +532,7 @@ void launch(const at::Tensor& logits, int V, const at::Tensor& ids, int64_t voca
   // CTAs per row: enough to fill four CTAs per SM, as long as each keeps a load per warp in flight
   int C = 1;
   while (C < MAX_CLUSTER && rows * C * 2 <= (int64_t)prop->multiProcessorCount * 4 && units >= C * 2 * WARPS) C *= 2;
-  const size_t smem = K > 0 ? sizeof(uint32_t) * ((units + C - 1) / C + 2) : 0;
+  const size_t smem = STAGES * STAGE_BYTES + (K > 0 ? sizeof(float) * ((units + C - 1) / C + 2 * WARPS) : 0);
   TORCH_CHECK(smem <= 200 * 1024, "token_logprobs: vocabulary of ", V, " is too wide for top_k");
   // the grid's y axis holds 65535 rows: longer batches go in several launches
   for (int64_t r0 = 0; r0 < rows; r0 += 65535) {
@@ -370,43 +553,50 @@ void launch(const at::Tensor& logits, int V, const at::Tensor& ids, int64_t voca
     cfg.numAttrs = snb::pdl_enabled() ? 2 : 1;
     const T* x = reinterpret_cast<const T*>(logits.data_ptr()) + r0 * logits.stride(0);
     const int64_t* id = ids.data_ptr<int64_t>() + r0;
+    float* out = stats.data_ptr<float>() + r0;
     float* tv = K > 0 ? top_vals.data_ptr<float>() + r0 * K : nullptr;
     int64_t* ti = K > 0 ? top_ids.data_ptr<int64_t>() + r0 * K : nullptr;
     auto kern = K > 0 ? logits_stats_kernel<T, true> : logits_stats_kernel<T, false>;
-    if (smem > 16 * 1024)
-      C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, x, logits.stride(0), V, id, vocab_offset, K,
-                                      logprobs.data_ptr<float>() + r0, entropy.data_ptr<float>() + r0,
-                                      lse.data_ptr<float>() + r0, tv, ti));
+                                      out, out + rows, out + 2 * rows, tv, ti, status));
   }
 }
 
 }  // namespace
 
 // logits: [N, >= V] bf16 / fp16 / fp32, any row stride; only the first V columns are read, whatever the rest holds.
-// ids: [N] int64 (less vocab_offset outside [0, V): log-probability -inf). Outputs: [N] fp32, top [N, K].
-void logits_stats(at::Tensor logits, int64_t V, at::Tensor ids, int64_t vocab_offset, int64_t K,
-                  at::Tensor logprobs, at::Tensor entropy, at::Tensor lse, at::Tensor top_vals,
-                  at::Tensor top_ids) {
+// ids: [N] int64 (less vocab_offset outside [0, V): log-probability -inf). Returns fp32 [3, N] (log-probability,
+// entropy, log-sum-exp), the K best log-probabilities [N, K] and their ids.
+std::tuple<at::Tensor, at::Tensor, at::Tensor> logits_stats(at::Tensor logits, int64_t V, at::Tensor ids,
+                                                            int64_t vocab_offset, int64_t K,
+                                                            at::Tensor status) {
   TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && (logits.stride(1) == 1 || logits.size(1) == 1),
               "token_logprobs: logits must be a CUDA matrix with contiguous rows");
   TORCH_CHECK(V > 0 && V <= logits.size(1) && V < (int64_t(1) << 30), "token_logprobs: valid_vocab ", V,
               " outside the logits' ", logits.size(1), " columns");
   TORCH_CHECK(K >= 0 && K <= MAX_TOP && K <= V, "token_logprobs: top_k ", K, " not in [0, ", MAX_TOP, "]");
-  TORCH_CHECK(ids.scalar_type() == at::kLong && ids.is_contiguous() && ids.numel() == logits.size(0),
+  TORCH_CHECK(ids.is_cuda() && ids.scalar_type() == at::kLong && ids.is_contiguous() && ids.numel() == logits.size(0),
               "token_logprobs: one int64 id per row");
-  if (logits.size(0) == 0) return;
-  switch (logits.scalar_type()) {
-    case at::kFloat:
-      launch<float>(logits, (int)V, ids, vocab_offset, (int)K, logprobs, entropy, lse, top_vals, top_ids);
-      break;
-    case at::kBFloat16:
-      launch<__nv_bfloat16>(logits, (int)V, ids, vocab_offset, (int)K, logprobs, entropy, lse, top_vals, top_ids);
-      break;
-    case at::kHalf:
-      launch<__half>(logits, (int)V, ids, vocab_offset, (int)K, logprobs, entropy, lse, top_vals, top_ids);
-      break;
-    default:
-      TORCH_CHECK(false, "token_logprobs: dtype ", logits.scalar_type());
+  const int64_t N = logits.size(0);
+  auto stats = at::empty({3, N}, logits.options().dtype(at::kFloat));
+  auto top_vals = at::empty({N, K}, logits.options().dtype(at::kFloat));
+  auto top_ids = at::empty({N, K}, ids.options());
+  int* st = status.data_ptr<int>();
+  if (N > 0) {
+    switch (logits.scalar_type()) {
+      case at::kFloat:
+        launch<float>(logits, (int)V, ids, vocab_offset, (int)K, stats, top_vals, top_ids, st);
+        break;
+      case at::kBFloat16:
+        launch<__nv_bfloat16>(logits, (int)V, ids, vocab_offset, (int)K, stats, top_vals, top_ids, st);
+        break;
+      case at::kHalf:
+        launch<__half>(logits, (int)V, ids, vocab_offset, (int)K, stats, top_vals, top_ids, st);
+        break;
+      default:
+        TORCH_CHECK(false, "token_logprobs: dtype ", logits.scalar_type());
+    }
   }
+  return {stats, top_vals, top_ids};
 }

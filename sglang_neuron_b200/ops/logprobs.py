@@ -7,7 +7,7 @@ hold does not matter. With a vocabulary-sharded head every rank calls them on it
 as `vocab_offset` and `merge_shards` joins the ranks' results. Parity: the reference sampler's per-shard logsumexp
 and exact top-logprobs (sglang_neuron/sampling.py:212-470).
 """
-from typing import NamedTuple, Optional
+from typing import NamedTuple
 
 import torch
 
@@ -63,6 +63,10 @@ def _check(rows: int, cols: int, ids: torch.Tensor, top_k: int, valid_vocab: int
     return V
 
 
+def _long(ids: torch.Tensor) -> torch.Tensor:
+    return ids if ids.dtype == torch.int64 and ids.is_contiguous() else ids.long().contiguous()
+
+
 def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, top_k: int = 0, vocab_offset: int = 0,
                    valid_vocab: int = 0) -> TokenLogprobs:
     """`logits` [N, C] (bf16, fp16 or fp32; any row stride), `ids` [N]; see TokenLogprobs."""
@@ -73,15 +77,10 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, top_k: int = 0, voca
         return token_logprobs_ref(logits, ids, top_k, vocab_offset, V)
     if logits.dtype not in (torch.bfloat16, torch.float16, torch.float32):
         raise ValueError(f"token_logprobs takes bf16, fp16 or fp32 on CUDA, got {logits.dtype}")
-    N, dev = logits.shape[0], logits.device
     if logits.stride(1) != 1 and logits.shape[1] > 1:
         logits = logits.contiguous()
-    stats = torch.empty(3, N, dtype=torch.float32, device=dev)
-    tl = torch.empty(N, top_k, dtype=torch.float32, device=dev)
-    ti = torch.empty(N, top_k, dtype=torch.int64, device=dev)
-    kernels().logits_stats(logits, V, ids.long().contiguous(), vocab_offset, top_k, stats[0], stats[1], stats[2],
-                           tl, ti)
-    return TokenLogprobs(stats[0], stats[1], stats[2], tl, ti)
+    stats, tl, ti = kernels().logits_stats(logits, V, _long(ids), vocab_offset, top_k, _status_buf(logits.device))
+    return TokenLogprobs(*stats.unbind(0), tl, ti)
 
 
 def head_logprobs(hidden: torch.Tensor, weight, ids: torch.Tensor, vocab_offset: int = 0,
@@ -100,7 +99,7 @@ def head_logprobs(hidden: torch.Tensor, weight, ids: torch.Tensor, vocab_offset:
         return token_logprobs_ref(hidden.to(wide) @ w[:V].to(wide).t(), ids, 0, vocab_offset, V)
     if hidden.dtype not in (torch.bfloat16, torch.float16):
         raise ValueError(f"head_logprobs takes bf16 or fp16 on CUDA, got {hidden.dtype}")
-    N, H, dev = hidden.shape[0], hidden.shape[1], hidden.device
+    N, H = hidden.shape
     if H % 8:
         raise ValueError(f"head_logprobs needs a hidden size that is a multiple of 8, got {H}")
     tiled = False
@@ -111,11 +110,8 @@ def head_logprobs(hidden: torch.Tensor, weight, ids: torch.Tensor, vocab_offset:
         hidden = hidden.contiguous()
     if not tiled and (weight.stride(1) != 1 or weight.stride(0) % 8 or weight.data_ptr() % 16):
         weight = weight.contiguous()
-    stats = torch.empty(3, N, dtype=torch.float32, device=dev)
-    kernels().head_stats(hidden, weight, V, tiled, ids.long().contiguous(), vocab_offset, stats[0], stats[1],
-                         stats[2], _status_buf(dev))
-    return TokenLogprobs(stats[0], stats[1], stats[2], stats.new_empty(N, 0),
-                         torch.empty(N, 0, dtype=torch.int64, device=dev))
+    stats = kernels().head_stats(hidden, weight, V, tiled, _long(ids), vocab_offset, _status_buf(hidden.device))
+    return TokenLogprobs(*stats.unbind(0), stats.new_empty(N, 0), ids.new_empty(N, 0, dtype=torch.int64))
 
 
 def merge_shards(shards) -> TokenLogprobs:

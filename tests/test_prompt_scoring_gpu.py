@@ -476,3 +476,28 @@ def test_prompt_attention_all_scores_minus_infinity():
         seen = prompt_attention(q[50:], k[50:], v[50:], _indptr([n - 50]), Hq, Hkv, D, sinks=sinks)
         tol = (4 * U[torch.bfloat16] + 8e-4) * v.float().abs().max().item()
         assert ((out[50:].float() - seen.float()).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("N", [2, 600])
+def test_token_logprobs_low_rows(dtype, N):
+    """Rows near the type's lowest value, with a few logits above it, and with -inf beside it; huge positive rows."""
+    from sglang_neuron_b200.ops.logprobs import token_logprobs
+    V, lo = 5003, torch.finfo(dtype).min
+    g = torch.Generator(device=DEV).manual_seed(N)
+    ids = torch.randint(0, V, (N,), device=DEV, generator=g)
+    step = 64.0 if dtype == torch.float16 else abs(lo) / 64
+    x = torch.full((N, V), lo, device=DEV, dtype=dtype)
+    x[:, ::7] = lo + step
+    x[:, 1::9] = -math.inf
+    _check_stats(token_logprobs(x, ids, top_k=4), x, ids, 4)
+    x[:, 4000] = 0.5
+    x[:, 17] = -1.25
+    _check_stats(token_logprobs(x, ids, top_k=4), x, ids, 4)
+    y = (torch.randn(N, V, device=DEV, generator=g) * 3).to(dtype)
+    y[:, ::2] = lo
+    y[:, 1::4] = -math.inf
+    _check_stats(token_logprobs(y, ids, top_k=20), y, ids, 20)
+    hi = torch.full((N, V), 6e4 if dtype == torch.float16 else 2e38, device=DEV, dtype=dtype)
+    hi[:, ::3] = 1.0
+    _check_stats(token_logprobs(hi, ids, top_k=2), hi, ids, 2)
