@@ -36,7 +36,6 @@ constexpr int STAGES = 3;
 constexpr int PER = 4;                    // segments that a warp reads of a stage
 constexpr int STAGE_UNITS = PER * WARPS;
 constexpr int STAGE_BYTES = STAGE_UNITS * 512;
-constexpr int AHEAD = 4;        // selected segments that a warp reads again at a time
 constexpr int MAX_TOP = 32;     // one entry per lane of a warp's sorted list
 constexpr int MAX_CLUSTER = 8;  // the portable cluster size
 constexpr float LOG2E = 1.4426950408889634f;
@@ -387,51 +386,66 @@ __global__ void __launch_bounds__(THREADS, 4)
     }
     // every warp sorts the entries >= thr of its own segments into a list held across its lanes
     uint64_t list = 0;
-    auto offer = [&](bool have, float v, uint32_t i) {
-      const uint32_t k32 = order_key(v);
-      if (!__ballot_sync(0xffffffffu, have && k32 >= thr)) return;
-      const uint64_t key = have ? ((uint64_t)k32 << 32) | (0xffffffffu - i) : 0ull;
-      const uint64_t kth = __shfl_sync(0xffffffffu, list, K - 1);
-      unsigned hit = __ballot_sync(0xffffffffu, key > kth && k32 >= thr);
-      while (hit) {
-        const int src = __ffs(hit) - 1;
-        hit &= hit - 1;
-        const uint64_t k = __shfl_sync(0xffffffffu, key, src);
-        const uint64_t up = __shfl_up_sync(0xffffffffu, list, 1);
-        if (k > list) list = (lane > 0 && k > up) ? up : k;
-      }
+    auto insert = [&](uint32_t k32, uint32_t i) {  // the same arguments in every lane
+      const uint64_t k = ((uint64_t)k32 << 32) | (0xffffffffu - i);
+      const uint64_t up = __shfl_up_sync(0xffffffffu, list, 1);
+      if (k > list) list = (lane > 0 && k > up) ? up : k;
     };
     const int mine_n = warp < WARPS && u1 - u0 - warp > 0 ? (u1 - u0 - warp + 2 * WARPS - 1) / (2 * WARPS) : 0;
 #pragma unroll 1
     for (int j0 = 0; j0 < mine_n; j0 += 32) {
       const int j = j0 + lane;
       unsigned sel = __ballot_sync(0xffffffffu, j < mine_n && order_key(seg_max[warp + j * WARPS]) >= thr);
+#pragma unroll 1
       while (sel) {
-        uint4 raw[AHEAD];
-        int iv[AHEAD];
+        uint4 raw[2];  // a segment is two of the warp's units
+        int un[2];
 #pragma unroll
-        for (int n = 0; n < AHEAD; ++n) {  // a segment is two of the warp's units
-          const int un = sel ? u0 + warp + (2 * (j0 + __ffs(sel) - 1) + n % 2) * WARPS : u1;
-          iv[n] = un < u1 ? un * 32 + lane : cut.nvec;
-          if (n % 2) sel &= sel - 1;
-          raw[n] = make_uint4(0, 0, 0, 0);
-          if (iv[n] < cut.nvec) raw[n] = __ldg(body + iv[n]);
+        for (int n = 0; n < 2; ++n) {
+          un[n] = u0 + warp + (2 * (j0 + __ffs(sel) - 1) + n) * WARPS;
+          raw[n] = make_uint4(Vec<T>::NONE, Vec<T>::NONE, Vec<T>::NONE, Vec<T>::NONE);
+          if (un[n] < u1 && un[n] * 32 + lane < cut.nvec) raw[n] = __ldg(body + un[n] * 32 + lane);
         }
+        sel &= sel - 1;
 #pragma unroll
-        for (int n = 0; n < AHEAD; ++n) {
-          const bool have = iv[n] < cut.nvec;
-          if (!__any_sync(0xffffffffu, have)) continue;
-          const uint32_t i0 = (uint32_t)(cut.head + iv[n] * N);
+        for (int n = 0; n < 2; ++n) {
+          if (un[n] >= u1) break;
+          // entries come in ascending order of their ids, so one that equals the K-th of a full list stays out
+          const uint64_t kth = __shfl_sync(0xffffffffu, list, K - 1);
+          const bool full_nan = (uint32_t)(kth >> 32) == 0xffffffffu;  // nothing orders above a NaN
+          const uint32_t least = kth ? max(thr, (uint32_t)(kth >> 32) + 1u) : thr;
+          unsigned bits = 0;
+          if (un[n] * 32 + lane < cut.nvec && !full_nan) {
 #pragma unroll
-          for (int i = 0; i < N / 2; ++i) {
-            const float2 v = Vec<T>::two(raw[n], i);
-            offer(have, v.x, i0 + 2 * i);
-            offer(have, v.y, i0 + 2 * i + 1);
+            for (int i = 0; i < N / 2; ++i) {
+              const float2 v = Vec<T>::two(raw[n], i);
+              bits |= (unsigned)(order_key(v.x) >= least) << (2 * i) | (unsigned)(order_key(v.y) >= least) << (2 * i + 1);
+            }
+          }
+          unsigned from = __ballot_sync(0xffffffffu, bits != 0);
+#pragma unroll 1
+          while (from) {
+            const int src = __ffs(from) - 1;
+            from &= from - 1;
+            unsigned m = __shfl_sync(0xffffffffu, bits, src);
+            const uint4 r = make_uint4(__shfl_sync(0xffffffffu, raw[n].x, src), __shfl_sync(0xffffffffu, raw[n].y, src),
+                                       __shfl_sync(0xffffffffu, raw[n].z, src), __shfl_sync(0xffffffffu, raw[n].w, src));
+#pragma unroll 1
+            for (; m; m &= m - 1) {
+              const int i = __ffs(m) - 1;
+              const float2 v = Vec<T>::two(r, i / 2);
+              insert(order_key(i & 1 ? v.y : v.x), (uint32_t)(cut.head + (un[n] * 32 + src) * N + i));
+            }
           }
         }
       }
     }
-    if (warp == 0) offer(mine, end_v, (uint32_t)end_i);
+    if (warp == 0) {
+      for (unsigned e = __ballot_sync(0xffffffffu, mine); e; e &= e - 1) {
+        const int src = __ffs(e) - 1;
+        insert(order_key(__shfl_sync(0xffffffffu, end_v, src)), (uint32_t)__shfl_sync(0xffffffffu, end_i, src));
+      }
+    }
     const bool valid = lane < K && list != 0;
     const unsigned vm = __ballot_sync(0xffffffffu, valid);
     int base = 0;
