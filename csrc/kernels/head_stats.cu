@@ -1,6 +1,12 @@
 // Log-probabilities of given tokens, entropy and log-sum-exp of an LM head's logits that are never stored:
 //   z[n, v] = sum_k hidden[n, k] weight[v, k]   (bf16 / fp16 operands, fp32 in tensor memory)
 //   y = z - c,  s = sum_v e^y,  t = sum_v e^y y    lse = c + log s   entropy = log s - t / s
+// A product kernel writes (c, s, t) of every vocabulary tile and row, head_join_kernel joins them.
+//
+// More than 128 rows: head_stats_kernel, bound by the tensor cores (under load by the GPU's power): 4096 x 4096 x
+// 151936 took 3123 us, 1632 TFLOP/s, where the library's product alone, in the same run, took 3219 us; 1000 x 2880 x
+// 201088 took 783 us (787 us). Up to 128 rows: head_few_kernel, bound by the weights' stream: 16 x 4096 x 151936 took
+// 219 us, 5.7 TB/s (the library's product: 211 us); at 129 rows the pair kernel takes 231 us, at 128 this one 228 us.
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <ATen/cuda/CUDAContext.h>

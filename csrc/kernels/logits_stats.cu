@@ -18,6 +18,9 @@
 // -6e4) keeps 0 * y finite where a logit is masked; a CTA whose every logit lies down there reads its part once more
 // on an exact path.
 // The row comes through a ring of three 16 KB bulk copies that one thread keeps full.
+// Measured on a B200: 4096 x 151936 bf16 without alternatives 224-243 us (5.1-5.5 TB/s), with five 261 us, with twenty
+// 294 us (choosing them is some 10 us per row, under other rows' streams); 1000 x 201088 fp32 with five 146 us (5.5
+// TB/s); 64 x 201088 fp32 with twenty 29 us, a single bf16 row with five 12 us, without 7 us.
 // Split: one CTA per row, four resident per SM; fewer rows than that put a cluster of 2 to 8 CTAs on each row, whose
 // partial results the first CTA joins through distributed shared memory.
 #include <ATen/core/Tensor.h>

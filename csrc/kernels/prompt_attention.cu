@@ -2,6 +2,20 @@
 //
 //   out[t, h] = sum_j p_j v[j, h / G],   p_j = exp(scale q[t, h] . k[j, h / G] - m) / (exp(sink[h] - m) + sum_j ...)
 //   over the tokens j <= t of the same prompt, t - j < window where a window is set.
+//
+// One pass over the keys in blocks of 128 with a running reference m and sum. A persistent CTA per SM works on two
+// query tiles of 128 rows that share their keys and values: scores S = Q K^T and output O += P V on tcgen05 with S, P
+// and O in tensor memory (P over the S it came from: 2 x (128 + 128) columns at head width 128), Q, K and V by TMA.
+// 16 softmax warps: two threads per row, 64 keys each.
+//
+// What bounds it: the softmax warps. A block of both tiles is 2048 cycles of tensor core at head width 128 and takes
+// about 2600; per score they spend 0.75 exponentials of the special-function unit's 1/4 a cycle and scheduler (the rest
+// runs on the FMA pipe), the packing to 16 bits and the sums. Measured on a B200 (device time): one 8192-token prompt,
+// 32 / 8 heads of 128: 430 us, 1279 TFLOP/s; 64 / 8 heads of 64: 650 us, 846 TFLOP/s (the same scores at half the
+// products); 16 heads of 192 / 128: 334 us, 1031 TFLOP/s.
+// Tried and slower: one thread per row (its chain of loads, maximum, exponentials is twice as long: 575 us); turns of
+// the two tiles at the exponentials (with one thread per row 4 % faster, with two a loss); heads of 64 with one tile
+// per CTA and two CTAs per SM (687 us against 650).
 #include <ATen/core/Tensor.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAException.h>
@@ -12,10 +26,9 @@
 
 namespace {
 
-#ifndef EMULATE_N
-#define EMULATE_N 4
-#endif
-constexpr int EMULATE = EMULATE_N;  // one pair of exponentials in this many runs on the FMA pipe
+// One pair of exponentials in this many runs on the FMA pipe. Cycles per block of both tiles at head width 128 with
+// one pair in 2, 3, 4, 8 and none: 2560, 2530, 2600, 2700, 3300.
+constexpr int EMULATE = 4;
 constexpr float LOG2E = 1.4426950408889634f;
 
 SNB_DEVICE float ex2(float x) {
@@ -392,9 +405,9 @@ __global__ void __launch_bounds__(THREADS, 1)
   if (warp == LOAD_WARP) {
     int nq = 0, nk = 0, nv = 0;
     bool ok = true;
-    // It alone works the items out (a few global reads and divisions), ahead of the warps that it hands them to.
-    for (int r = 0; ok; ++r) {
-      Item it;
+    // It alone works the items out (a few global reads and divisions) and hands them over one item ahead, before it
+    // waits for the ring.
+    auto publish = [&](int r, Item& it) {
       const bool have = next_item(p, r, it);
       if (!have) it.kb0 = it.kb1 = 0;
       if (lane == 0) {
@@ -404,7 +417,13 @@ __global__ void __launch_bounds__(THREADS, 1)
           snb::mbar_arrive(&i_full[r & 1]);
         }
       }
-      if (!have) break;
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+      return have;
+    };
+    Item it, next;
+    bool have = publish(0, it);
+    for (int r = 0; ok && have; ++r, it = next) {
+      have = publish(r + 1, next);
       if (lane == 0 && ok) {
         const int hk = it.h0 / G;
         auto load_k = [&](int kb) {
@@ -427,7 +446,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           ++nv;
           return true;
         };
-        ok = snb::mbar_wait_bounded(q_empty, (nq & 1) ^ 1, status, SNB_ERR_TIMEOUT_TMA);
+        ok = load_k(it.kb0) && snb::mbar_wait_bounded(q_empty, (nq & 1) ^ 1, status, SNB_ERR_TIMEOUT_TMA);
         if (ok) {
           snb::mbar_arrive_expect_tx(q_full, 2 * C::QB);
 #pragma unroll
@@ -437,7 +456,7 @@ __global__ void __launch_bounds__(THREADS, 1)
               snb::tma_load_2d(sQ + j * C::QB + c * CHUNK, &tq, q_full, (it.h0 + (p.pair_heads ? j : 0)) * D + c * 64,
                                it.first + it.r0 + (p.pair_heads ? 0 : j * BQ));
           ++nq;
-          for (int kb = it.kb0; ok && kb < it.kb1; ++kb) ok = load_k(kb) && load_v(kb);
+          for (int kb = it.kb0; ok && kb < it.kb1; ++kb) ok = load_v(kb) && (kb + 1 == it.kb1 || load_k(kb + 1));
         }
       }
       ok = __shfl_sync(0xffffffffu, ok, 0);
@@ -630,7 +649,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           else maximum(std::false_type());
           const float top = fmaxf(mx[0], mx[1]) * p.scale;
           const bool rise = m == -INFINITY ? top > m : top - m > 8.f;
-          if (bar_or(bar, rise || !ok)) {
+          if (!NARROW || bar_or(bar, rise || !ok)) {
             if (bar_or(bar, !ok)) {
               ok = false;
               break;
@@ -666,8 +685,11 @@ __global__ void __launch_bounds__(THREADS, 1)
                   e.x = ex2(e.x);
                   e.y = ex2(e.y);
                 }
-                sum[i & 1] = add2(sum[i & 1], pair(e.x, e.y));
                 w2[i] = pack2<T>(e.x, e.y);
+                // a row of few keys (it sees all of them in ragged blocks) sums the weights as rounded: what the
+                // product uses then adds up to one
+                if (cut.value) e = unpack2<T>(w2[i]);
+                sum[i & 1] = add2(sum[i & 1], pair(e.x, e.y));
               }
             }
             tmem_st_x8(s_at + c * 8, w2);

@@ -5,6 +5,7 @@
     python -m sglang_neuron_b200.benchmarks.kernels gemm --tokens 64 --n 5120 --k 2880
     python -m sglang_neuron_b200.benchmarks.kernels attn --batch 64 --ctx 1536
     python -m sglang_neuron_b200.benchmarks.kernels mla --batch 32 --ctx 4096       # DeepSeek-V2-Lite MLA
+    python -m sglang_neuron_b200.benchmarks.kernels score --tokens 4096 --hq 32 --hkv 8 --head-dim 128   # prompt scoring
 
 Peaks come from MEASURED_PEAKS.json at the repository root when present (hbm_gbs, bf16_tflops), else the
 pool's fallback figures (6650 GB/s, 1590 TFLOP/s). Pass --iters 1 --warmup 1 for a profiler capture.
@@ -290,9 +291,35 @@ def bench_mla(a):
     print(json.dumps(res))
 
 
+def bench_score(a):
+    """The operators of Engine.score on one prompt of --tokens tokens: attention of a layer, the head's statistics
+    straight from the hidden rows, and from logits with five alternatives."""
+    from ..ops.logprobs import head_logprobs, token_logprobs
+    from ..ops.prompt import prompt_attention
+    T, Hq, Hkv, D, H, V = a.tokens, a.hq, a.hkv, a.head_dim, 4096, 151936
+    hbm, tf, src = peaks()
+    qkv = torch.randn(T, (Hq + 2 * Hkv) * D, device="cuda").to(torch.bfloat16)
+    q, k, v = qkv.split([Hq * D, Hkv * D, Hkv * D], dim=1)
+    bounds = torch.tensor([0, T], dtype=torch.int32, device="cuda")
+    us = timeit(lambda: prompt_attention(q, k, v, bounds, Hq, Hkv, D), a.iters, a.warmup)
+    fl = 2.0 * T * (T + 1) * Hq * D
+    res = {"kernel": "prompt scoring", "tokens": T, "heads": f"{Hq}/{Hkv}x{D}", "attention_us": round(us, 1),
+           f"attention_frac_of_{src}_bf16": round(fl / us / 1e6 / tf, 3)}
+    h = torch.randn(T, H, device="cuda").to(torch.bfloat16)
+    w = (torch.randn(V, H, device="cuda") * 0.02).to(torch.bfloat16)
+    ids = torch.randint(0, V, (T,), device="cuda")
+    us = timeit(lambda: head_logprobs(h, w, ids), a.iters, a.warmup)
+    res.update({"head_us": round(us, 1), f"head_frac_of_{src}_bf16": round(2.0 * T * H * V / us / 1e6 / tf, 3),
+                f"head_frac_of_{src}_hbm": round(2.0 * H * (T + V) / us / 1e3 / hbm, 3)})
+    x = torch.nn.functional.linear(h, w)
+    us = timeit(lambda: token_logprobs(x, ids, top_k=5), a.iters, a.warmup)
+    res.update({"logits_us": round(us, 1), f"logits_frac_of_{src}_hbm": round(2.0 * T * V / us / 1e3 / hbm, 3)})
+    print(json.dumps(res))
+
+
 def main():
     p = argparse.ArgumentParser()
-    p.add_argument("which", choices=["moe", "moe_stages", "route", "gemm", "attn", "mla"])
+    p.add_argument("which", choices=["moe", "moe_stages", "route", "gemm", "attn", "mla", "score"])
     p.add_argument("--ep", type=int, default=1)
     p.add_argument("--bn", type=int, default=0, help="moe_stages: force the token tile (16/32/64/128)")
     p.add_argument("--only", default="", help="moe_stages: comma-separated stages to time")
@@ -314,7 +341,7 @@ def main():
     p.add_argument("--warmup", type=int, default=3)
     a = p.parse_args()
     {"moe": bench_moe, "moe_stages": bench_moe_stages, "route": bench_route, "gemm": bench_gemm,
-     "attn": bench_attn, "mla": bench_mla}[a.which](a)
+     "attn": bench_attn, "mla": bench_mla, "score": bench_score}[a.which](a)
 
 
 if __name__ == "__main__":
