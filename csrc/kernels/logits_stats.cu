@@ -8,7 +8,7 @@
 //
 // The best K entries (value descending, ties to the lower id) come from the same pass: a warp reads 512 contiguous
 // bytes per load and keeps the maximum of every two loads (a segment), which the running reference needs anyway. The K-th
-// best of the threads' maxima is a lower bound of the K-th best entry, so afterwards only the segments whose
+// best of 32 groups' maxima is a lower bound of the K-th best entry, so afterwards only the segments whose
 // maximum reaches it are read again (they are in L2) and sorted in by (value, ~id) keys: about K segments for
 // ordinary rows, all of them for a constant row.
 //
@@ -170,18 +170,12 @@ struct Stats {
   float c, s, t;  // reference, sum of e^y, sum of e^y y
 };
 
-SNB_DEVICE Stats join(const Stats& a, const Stats& b) {
-  if (a.c == -INFINITY) return b;  // nothing seen yet
-  if (b.c == -INFINITY) return a;
-  const float C = max_nan(a.c, b.c);
-  const float fa = ex2((a.c - C) * LOG2E), fb = ex2((b.c - C) * LOG2E);
-  Stats r;
-  r.c = C;
-  r.s = a.s * fa + b.s * fb;
-  // the far side's weight is 0 when its distance is infinite or merely large: 0 * inf must not become NaN
-  r.t = (fa > 0.f ? fa * (a.t + a.s * (a.c - C)) : 0.f) + (fb > 0.f ? fb * (b.t + b.s * (b.c - C)) : 0.f);
-  if (C != C || C == INFINITY) r.s = r.t = NAN;
-  return r;
+// Sums over the first `W` lanes (a power of two), in every one of them
+template <int W>
+SNB_DEVICE float lane_sum(float v) {
+#pragma unroll
+  for (int o = W / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
 }
 
 // A row is cut into an unaligned head (fewer than one vector), `units` segments of 32 vectors, and a tail.
@@ -208,8 +202,9 @@ __global__ void __launch_bounds__(THREADS, 4)
   extern __shared__ __align__(128) uint8_t dyn[];  // the ring, then the segments' maxima
   float* seg_max = reinterpret_cast<float*>(dyn + STAGES * STAGE_BYTES);
   __shared__ uint64_t full[STAGES], empty[STAGES];
-  __shared__ Stats warp_stats[WARPS];
-  __shared__ float warp_best[WARPS + 1];
+  __shared__ float warp_s[WARPS], warp_t[WARPS], warp_best[WARPS + 1];
+  __shared__ uint32_t best_keys[WARPS * 32];
+  __shared__ float row_c, row_lg;
   __shared__ Stats cta_stats[MAX_CLUSTER];
   __shared__ uint64_t cand[WARPS * MAX_TOP];
   __shared__ uint64_t lists[MAX_CLUSTER * MAX_TOP];  // filled by every CTA of the cluster in the first one's memory
@@ -267,6 +262,8 @@ __global__ void __launch_bounds__(THREADS, 4)
 
   const int v0 = u0 * 32, v1 = min(u1 * 32, cut.nvec);  // this CTA's vectors
   const int stages = (u1 - u0 + STAGE_UNITS - 1) / STAGE_UNITS;
+  bool given = false;  // the given token's logit, in the last warp's first lane
+  float given_x = 0.f;
   if (warp == WARPS) {
     if (lane == 0) {
       int i = 0;
@@ -281,6 +278,9 @@ __global__ void __launch_bounds__(THREADS, 4)
       // nothing is in flight when the memory goes away, even if the readers gave up
       for (int d = max(0, i - STAGES); d < i; ++d)
         snb::mbar_wait_bounded(&full[d % STAGES], (d / STAGES) & 1, status, SNB_ERR_TIMEOUT_TMA);
+      const int64_t id = ids[row] - vocab_offset;
+      given = id >= 0 && id < V;
+      if (given) given_x = Vec<T>::one(x[id]);
     }
     __syncwarp();
   } else {
@@ -331,19 +331,13 @@ __global__ void __launch_bounds__(THREADS, 4)
 #pragma unroll
   for (int i = 1; i <= WARPS; ++i) most = max_nan(most, warp_best[i]);
 
-  // to natural units, against the thread's own maximum: cl is its product with log2 e, rounded
-  Stats st{-INFINITY, 0.f, 0.f};
+  // From here on against the CTA's maximum, in natural units. A sum that weighs nothing there must not meet an infinite
+  // distance; where the maximum is NaN the row is NaN whatever the sums are.
+  float st_s = 0.f, st_t = 0.f;
   auto exact = [&](float v) {
-    if (v == -INFINITY) return;
-    if (v > st.c || v != v) {
-      const float f = ex2((st.c - v) * LOG2E);
-      st.t = f > 0.f ? f * (st.t + st.s * (st.c - v)) : 0.f;
-      st.s *= f;
-      st.c = v;
-    }
-    const float y = max_nan(v - st.c, -1e30f), e = ex2(y * LOG2E);
-    st.s += e;
-    st.t = fmaf(e, y, st.t);
+    const float y = max_nan(v - most, -1e30f), e = ex2(y * LOG2E);
+    st_s += e;
+    st_t = fmaf(e, y, st_t);
   };
   if (most <= Vec<T>::LOWEST || most > 1e30f) {
     if (warp < WARPS && most != -INFINITY)
@@ -357,36 +351,33 @@ __global__ void __launch_bounds__(THREADS, 4)
           exact(v.y);
         }
       }
-  } else if (!(cl <= Vec<T>::FLOOR * LOG2E)) {
+  } else {
     const float2 ss = split(s2), ts = split(t2);
-    st.c = cl * (1.f / LOG2E);
-    const float off = fmaf(-st.c, LOG2E, cl), f = ex2(off);
-    st.s = (ss.x + ss.y) * f;
-    st.t = ((ts.x + ts.y) + (ss.x + ss.y) * off) * f * LN2;
+    const float d = fmaf(-most, LOG2E, cl), f = ex2(d);
+    if (f > 0.f) {
+      st_s = (ss.x + ss.y) * f;
+      st_t = fmaf(ss.x + ss.y, d, ts.x + ts.y) * f * LN2;
+    }
   }
-  if (mine) exact(end_v);
-
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    Stats b;
-    b.c = __shfl_xor_sync(0xffffffffu, st.c, o);
-    b.s = __shfl_xor_sync(0xffffffffu, st.s, o);
-    b.t = __shfl_xor_sync(0xffffffffu, st.t, o);
-    // both lanes of a pair join in the same order: every lane ends with the same bits
-    st = (lane & o) ? join(b, st) : join(st, b);
+  if (mine && most != -INFINITY) exact(end_v);
+  st_s = lane_sum<32>(st_s);
+  st_t = lane_sum<32>(st_t);
+  if (warp < WARPS) {
+    if (lane == 0) warp_s[warp] = st_s, warp_t[warp] = st_t;
+    if (TOP) best_keys[threadIdx.x] = any ? order_key(best) : 0u;
   }
-  if (lane == 0 && warp < WARPS) warp_stats[warp] = st;
+  __syncthreads();
 
   if constexpr (TOP) {
-    // a lower bound of the K-th best entry: the K-th largest of the threads' maxima, to the upper 16 bits of its key
-    // (0 when fewer than K threads hold any entry)
-    const uint32_t best_key = any ? order_key(best) : 0u;
-    uint32_t thr = 0;
-#pragma unroll 1
-    for (int b = 31; b >= 16; --b) {
-      const uint32_t t = thr | (1u << b);
-      if (__syncthreads_count(best_key >= t) >= K) thr = t;
-    }
+    // a lower bound of the K-th best entry: the K-th largest of 32 groups' maxima, a group being the threads of one
+    // lane number (0 when fewer than K groups hold any entry); every warp finds it for itself
+    uint32_t g = 0;
+#pragma unroll
+    for (int i = 0; i < WARPS; ++i) g = max(g, best_keys[i * 32 + lane]);
+    int above = 0;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) above += __shfl_sync(0xffffffffu, g, i) > g;
+    const uint32_t thr = __reduce_min_sync(0xffffffffu, above < K ? g : 0xffffffffu);
     // every warp sorts the entries >= thr of its own segments into a list held across its lanes
     uint64_t list = 0;
     auto insert = [&](uint32_t k32, uint32_t i) {  // the same arguments in every lane
@@ -401,18 +392,18 @@ __global__ void __launch_bounds__(THREADS, 4)
       unsigned sel = __ballot_sync(0xffffffffu, j < mine_n && order_key(seg_max[warp + j * WARPS]) >= thr);
 #pragma unroll 1
       while (sel) {
-        uint4 raw[2];  // a segment is two of the warp's units
-        int un[2];
+        uint4 raw[4];  // two segments, each two of the warp's units
+        int un[4];
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          un[n] = u0 + warp + (2 * (j0 + __ffs(sel) - 1) + n) * WARPS;
+        for (int n = 0; n < 4; ++n) {
+          un[n] = sel ? u0 + warp + (2 * (j0 + __ffs(sel) - 1) + n % 2) * WARPS : u1;
+          if (n % 2) sel &= sel - 1;
           raw[n] = make_uint4(Vec<T>::NONE, Vec<T>::NONE, Vec<T>::NONE, Vec<T>::NONE);
           if (un[n] < u1 && un[n] * 32 + lane < cut.nvec) raw[n] = __ldg(body + un[n] * 32 + lane);
         }
-        sel &= sel - 1;
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          if (un[n] >= u1) break;
+        for (int n = 0; n < 4; ++n) {
+          if (un[n] >= u1) continue;
           // entries come in ascending order of their ids, so one that equals the K-th of a full list stays out
           const uint64_t kth = __shfl_sync(0xffffffffu, list, K - 1);
           const bool full_nan = (uint32_t)(kth >> 32) == 0xffffffffu;  // nothing orders above a NaN
@@ -460,16 +451,11 @@ __global__ void __launch_bounds__(THREADS, 4)
 
   // this CTA's result, into the first CTA's shared memory
   uint32_t dst_rank = 0;
-  if (warp == 0) {
-    Stats a = lane < WARPS ? warp_stats[lane] : Stats{-INFINITY, 0.f, 0.f};
-#pragma unroll
-    for (int o = WARPS / 2; o > 0; o >>= 1) {
-      Stats b;
-      b.c = __shfl_xor_sync(0xffffffffu, a.c, o);
-      b.s = __shfl_xor_sync(0xffffffffu, a.s, o);
-      b.t = __shfl_xor_sync(0xffffffffu, a.t, o);
-      a = (lane & o) ? join(b, a) : join(a, b);
-    }
+  if (warp == WARPS) {  // the warp that has the least to do
+    Stats a;
+    a.c = most;
+    a.s = lane_sum<WARPS>(lane < WARPS ? warp_s[lane] : 0.f);
+    a.t = lane_sum<WARPS>(lane < WARPS ? warp_t[lane] : 0.f);
     if (lane == 0) {
       const uint32_t at = snb::mapa_shared(snb::smem_u32(&cta_stats[rank]), dst_rank);
       asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(a.c) : "memory");
@@ -482,6 +468,7 @@ __global__ void __launch_bounds__(THREADS, 4)
     for (int i = threadIdx.x; i < n; i += THREADS) {
       const uint64_t k = cand[i];
       int r = 0;
+#pragma unroll 8
       for (int j = 0; j < n; ++j) r += cand[j] > k;
       if (r < K) {
         const uint32_t at = snb::mapa_shared(snb::smem_u32(&lists[rank * MAX_TOP + r]), dst_rank);
@@ -501,26 +488,34 @@ __global__ void __launch_bounds__(THREADS, 4)
     __syncthreads();
   }
 
-  // every thread of the first CTA joins the few partial results itself
-  Stats a = cta_stats[0];
-  for (int r = 1; r < C; ++r) a = join(a, cta_stats[r]);
-  const bool none = a.c == -INFINITY;  // every logit is -inf
-  const float lg = logf(a.s);
-  const float lse = none ? -INFINITY : a.c + lg;
-  if (threadIdx.x == 0) {
-    const int64_t id = ids[row] - vocab_offset;
-    float lp = -INFINITY;
-    if (id >= 0 && id < V && !none) lp = (Vec<T>::one(x[id]) - a.c) - lg;
-    logprobs[row] = lp;
-    entropy[row] = none ? 0.f : lg - a.t / a.s;
-    lse_out[row] = lse;
+  if (warp == WARPS) {
+    // two partial results join by their maximum: s' = s e^(c - C), t' = (t + s (c - C)) e^(c - C)
+    Stats a{-INFINITY, 0.f, 0.f};
+    if (lane < C) a = cta_stats[lane];
+    const float m = warp_max_nan(a.c), d = a.c - m, f = ex2(d * LOG2E);
+    const float ws = lane_sum<MAX_CLUSTER>(f > 0.f ? a.s * f : 0.f);
+    const float wt = lane_sum<MAX_CLUSTER>(f > 0.f ? (a.t + a.s * d) * f : 0.f);
+    if (lane == 0) {
+      const bool none = m == -INFINITY;  // every logit is -inf
+      const bool bad = m != m || m == INFINITY;
+      const float lg = bad ? NAN : logf(ws);
+      float lp = -INFINITY;
+      if (given && !none) lp = (given_x - m) - lg;
+      logprobs[row] = lp;
+      entropy[row] = none ? 0.f : lg - wt / ws;
+      lse_out[row] = none ? -INFINITY : m + lg;
+      row_c = m;
+      row_lg = lg;
+    }
   }
   if constexpr (TOP) {
-    for (int i = threadIdx.x; i < C * MAX_TOP; i += THREADS) {
-      const int r = i / MAX_TOP, p = i % MAX_TOP;
-      if (p >= best_n[r]) continue;
-      const uint64_t k = lists[i];
-      int at = p;  // the lists are sorted and their keys differ: the place in the merged list is the sum of ranks
+    // a merged list's places: the lists are sorted and their keys differ, so an entry's place is the sum of its ranks
+    const int i = threadIdx.x, r = i / MAX_TOP, p = i % MAX_TOP;
+    uint64_t k = 0;
+    int at = K;
+    if (r < C && p < best_n[r]) {
+      k = lists[i];
+      at = p;
       for (int q = 0; q < C; ++q) {
         if (q == r) continue;
         int lo = 0, hi = best_n[q];  // how many of list q come before
@@ -531,10 +526,11 @@ __global__ void __launch_bounds__(THREADS, 4)
         }
         at += lo;
       }
-      if (at < K) {
-        top_vals[row * K + at] = none ? -INFINITY : (key_value((uint32_t)(k >> 32)) - a.c) - lg;
-        top_ids[row * K + at] = vocab_offset + (int64_t)(0xffffffffu - (uint32_t)k);
-      }
+    }
+    __syncthreads();
+    if (at < K) {
+      top_vals[row * K + at] = row_c == -INFINITY ? -INFINITY : (key_value((uint32_t)(k >> 32)) - row_c) - row_lg;
+      top_ids[row * K + at] = vocab_offset + (int64_t)(0xffffffffu - (uint32_t)k);
     }
   }
 }
