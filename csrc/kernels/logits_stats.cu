@@ -18,9 +18,10 @@
 // -6e4) keeps 0 * y finite where a logit is masked; a CTA whose every logit lies down there reads its part once more
 // on an exact path.
 // The row comes through a ring of three 16 KB bulk copies that one thread keeps full.
-// Measured on a B200: 4096 x 151936 bf16 without alternatives 224-243 us (5.1-5.5 TB/s), with five 261 us, with twenty
-// 294 us (choosing them is some 10 us per row, under other rows' streams); 1000 x 201088 fp32 with five 146 us (5.5
-// TB/s); 64 x 201088 fp32 with twenty 29 us, a single bf16 row with five 12 us, without 7 us.
+// Measured on a B200: 4096 x 151936 bf16 without alternatives 235 us (5.3 TB/s), with five 262 us, with twenty 305 us
+// (choosing them takes a CTA some 5 us after its row); 1000 x 201088 fp32 with five 135 us (6.0 TB/s); 64 x 201088 fp32
+// without alternatives 14.5 us, with twenty 26 us; a single bf16 row with five 9 us, without 5 us. Tried and slower:
+// CTAs that stay and load the next row's first stages while they choose (280 us with five); the bound from 64 groups.
 // Split: one CTA per row, four resident per SM; fewer rows than that put a cluster of 2 to 8 CTAs on each row, whose
 // partial results the first CTA joins through distributed shared memory.
 #include <ATen/core/Tensor.h>
@@ -221,6 +222,8 @@ __global__ void __launch_bounds__(THREADS, 4)
     }
     snb::fence_mbar_init();
   }
+  // the first CTA's memory is written from the others: all of them have to be there by then
+  if (C > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   __syncthreads();
   snb::pdl_wait();
   snb::pdl_trigger();
@@ -450,7 +453,11 @@ __global__ void __launch_bounds__(THREADS, 4)
   __syncthreads();
 
   // this CTA's result, into the first CTA's shared memory
-  uint32_t dst_rank = 0;
+  const uint32_t dst_rank = 0;
+  if (C > 1) {
+    __syncwarp();
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+  }
   if (warp == WARPS) {  // the warp that has the least to do
     Stats a;
     a.c = most;
