@@ -74,16 +74,17 @@ void kv_page_slice_copy(torch::Tensor src_bases, torch::Tensor dst_bases, torch:
                         torch::Tensor dst_pages, int64_t src_page_bytes, int64_t dst_page_bytes, int64_t src_off,
                         int64_t dst_off, int64_t nbytes);
 // logits_stats.cu
-std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> logits_stats(torch::Tensor logits, int64_t V, torch::Tensor ids,
-                                                                     int64_t vocab_offset, int64_t K,
-                                                                     torch::Tensor status);
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor> logits_stats(
+    torch::Tensor logits, int64_t V, torch::Tensor ids, int64_t vocab_offset, int64_t K, torch::Tensor status);
 // head_stats.cu
-torch::Tensor head_stats(torch::Tensor hidden, torch::Tensor weight, int64_t V, bool tiled, torch::Tensor ids,
-                         int64_t vocab_offset, torch::Tensor status);
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> head_stats(torch::Tensor hidden, torch::Tensor weight,
+                                                                   int64_t F, bool tiled, int64_t V, torch::Tensor ids,
+                                                                   int64_t vocab_offset, torch::Tensor status);
 // prompt_attention.cu
-void prompt_attention(torch::Tensor out, torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor indptr,
-                      int64_t heads, int64_t kv_heads, int64_t D, int64_t DV, int64_t window, double sm_scale,
-                      c10::optional<torch::Tensor> sinks, torch::Tensor status);
+torch::Tensor prompt_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor indptr, int64_t heads,
+                               int64_t kv_heads, int64_t D, int64_t DV, int64_t window, double sm_scale,
+                               c10::optional<torch::Tensor> sinks, c10::optional<torch::Tensor> out,
+                               torch::Tensor status);
 int64_t nvls_flag_bytes();
 void nvls_allreduce(torch::Tensor out, torch::Tensor x, int64_t uc, int64_t mc, int64_t capacity, int64_t rank,
                     int64_t world, int64_t max_ctas, torch::Tensor status);

@@ -11,9 +11,11 @@
 #include <ATen/ops/empty.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAException.h>
+#include <c10/cuda/CUDAGuard.h>
 #include "../common.cuh"
 #include "../tma_host.h"
 #include <algorithm>
+#include <tuple>
 
 namespace {
 
@@ -569,20 +571,39 @@ int pick_width(int mt, int64_t V, int pairs) {
 
 }  // namespace
 
-// hidden [N, K], weight [>= V, K] (or 128 x 64 tiles, `tiled`), both bf16 or both fp16; ids [N] int64. Returns fp32
-// [3, N]: log-probability, entropy, log-sum-exp.
-at::Tensor head_stats(at::Tensor hidden, at::Tensor weight, int64_t V, bool tiled, at::Tensor ids,
-                      int64_t vocab_offset, at::Tensor status) {
+// hidden [N, K], weight [F, K] (or its 128 x 64 tiles, `tiled`, with F given), both bf16 or both fp16, K a multiple of
+// 8; the first V entries (V = 0: all) are the vocabulary. ids [N] int64 or int32. Returns fp32 [N] log-probability,
+// entropy and log-sum-exp.
+std::tuple<at::Tensor, at::Tensor, at::Tensor> head_stats(at::Tensor hidden, at::Tensor weight, int64_t F, bool tiled,
+                                                          int64_t V, at::Tensor ids, int64_t vocab_offset,
+                                                          at::Tensor status) {
+  // plain messages: putting numbers into them needs streams that this extension does not bring along
+  TORCH_CHECK(hidden.is_cuda() && hidden.dim() == 2 && weight.dim() == 2 &&
+                  (tiled || hidden.size(1) == weight.size(1)),
+              "head_logprobs: hidden [rows, size] does not fit the weight [vocabulary, size]");
   const int64_t N = hidden.size(0), K = hidden.size(1);
-  TORCH_CHECK(hidden.is_cuda() && hidden.stride(1) == 1 && weight.stride(1) == 1, "head_logprobs: row-major operands");
-  TORCH_CHECK(hidden.scalar_type() == weight.scalar_type() &&
-                  (hidden.scalar_type() == at::kBFloat16 || hidden.scalar_type() == at::kHalf),
-              "head_logprobs: bf16 or fp16 operands of one type");
-  TORCH_CHECK(ids.is_cuda() && ids.scalar_type() == at::kLong && ids.is_contiguous() && ids.numel() == N,
-              "head_logprobs: one int64 id per row");
-  TORCH_CHECK(K > 0 && V > 0 && V < (int64_t(1) << 30) && N < (int64_t(1) << 30), "head_logprobs: sizes");
+  if (!tiled) F = weight.size(0);
+  if (V == 0) V = F;
+  const auto type = hidden.scalar_type();
+  TORCH_CHECK(type == weight.scalar_type() && weight.device() == hidden.device(),
+              "head_logprobs: hidden and the weight differ in type or device");
+  TORCH_CHECK(type == at::kBFloat16 || type == at::kHalf, "head_logprobs: takes bf16 or fp16 on CUDA");
+  TORCH_CHECK(K > 0 && K % 8 == 0, "head_logprobs: needs a hidden size that is a multiple of 8");
+  TORCH_CHECK(V > 0 && V <= F && V < (int64_t(1) << 30), "head_logprobs: valid_vocab is outside the weight's rows");
+  TORCH_CHECK(ids.dim() == 1 && ids.numel() == N && ids.device() == hidden.device() &&
+                  (ids.scalar_type() == at::kLong || ids.scalar_type() == at::kInt),
+              "head_logprobs: ids must be one int64 or int32 per row on the rows' device");
+  TORCH_CHECK(N < (int64_t(1) << 30), "head_logprobs: too many rows");
+  const c10::cuda::CUDAGuard guard(hidden.device());
+  auto readable = [](const at::Tensor& x) {
+    return x.stride(1) == 1 && x.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
+  };
   auto stats = at::empty({3, N}, hidden.options().dtype(at::kFloat));
-  if (N == 0) return stats;
+  const auto result = std::make_tuple(stats.select(0, 0), stats.select(0, 1), stats.select(0, 2));
+  if (N == 0) return result;
+  if (!readable(hidden)) hidden = hidden.contiguous();
+  if (!readable(weight)) weight = weight.contiguous();
+  ids = ids.to(at::kLong).contiguous();
   const bool bf16 = hidden.scalar_type() == at::kBFloat16;
   const auto dt = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   auto st = at::cuda::getCurrentCUDAStream();
@@ -618,7 +639,7 @@ at::Tensor head_stats(at::Tensor hidden, at::Tensor weight, int64_t V, bool tile
     C10_CUDA_CHECK(cudaFuncSetAttribute(head_few_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
     C10_CUDA_CHECK(snb::launch_pdl(head_few_kernel, dim3(std::min(groups, sms)), dim3(THREADS), SMEM, st, th, tw, tw32, p));
     join_parts(part, p.chosen, (int)N, (int)N, (int)V, groups, GROUP, p.ids, vocab_offset, stats, st);
-    return stats;
+    return result;
   }
   const CUtensorMap th = snb_host::make_tmap_2d(hidden.data_ptr(), dt, K, N, hidden.stride(0) * 2, BK, BM,
                                                 CU_TENSOR_MAP_SWIZZLE_128B);
@@ -655,5 +676,5 @@ at::Tensor head_stats(at::Tensor hidden, at::Tensor weight, int64_t V, bool tile
   cfg.numAttrs = snb::pdl_enabled() ? 2 : 1;
   C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, head_stats_kernel, th, tw, p));
   join_parts(part, nullptr, n_pad, (int)N, (int)V, vt, width, p.ids, vocab_offset, stats, st);
-  return stats;
+  return result;
 }

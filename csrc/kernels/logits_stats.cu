@@ -28,6 +28,7 @@
 #include <ATen/ops/empty.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAException.h>
+#include <c10/cuda/CUDAGuard.h>
 #include "../common.cuh"
 #include <algorithm>
 #include <tuple>
@@ -553,7 +554,7 @@ void launch(const at::Tensor& logits, int V, const at::Tensor& ids, int64_t voca
   int C = 1;
   while (C < MAX_CLUSTER && rows * C * 2 <= (int64_t)prop->multiProcessorCount * 4 && units >= C * 2 * WARPS) C *= 2;
   const size_t smem = STAGES * STAGE_BYTES + (K > 0 ? sizeof(float) * ((units + C - 1) / C + 2 * WARPS) : 0);
-  TORCH_CHECK(smem <= 200 * 1024, "token_logprobs: vocabulary of ", V, " is too wide for top_k");
+  TORCH_CHECK(smem <= 200 * 1024, "token_logprobs: the vocabulary is too wide for top_k");
   // the grid's y axis holds 65535 rows: longer batches go in several launches
   for (int64_t r0 = 0; r0 < rows; r0 += 65535) {
     const int n = (int)std::min<int64_t>(65535, rows - r0);
@@ -585,38 +586,36 @@ void launch(const at::Tensor& logits, int V, const at::Tensor& ids, int64_t voca
 
 }  // namespace
 
-// logits: [N, >= V] bf16 / fp16 / fp32, any row stride; only the first V columns are read, whatever the rest holds.
-// ids: [N] int64 (less vocab_offset outside [0, V): log-probability -inf). Returns fp32 [3, N] (log-probability,
-// entropy, log-sum-exp), the K best log-probabilities [N, K] and their ids.
-std::tuple<at::Tensor, at::Tensor, at::Tensor> logits_stats(at::Tensor logits, int64_t V, at::Tensor ids,
-                                                            int64_t vocab_offset, int64_t K,
-                                                            at::Tensor status) {
-  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && (logits.stride(1) == 1 || logits.size(1) == 1),
-              "token_logprobs: logits must be a CUDA matrix with contiguous rows");
-  TORCH_CHECK(V > 0 && V <= logits.size(1) && V < (int64_t(1) << 30), "token_logprobs: valid_vocab ", V,
-              " outside the logits' ", logits.size(1), " columns");
-  TORCH_CHECK(K >= 0 && K <= MAX_TOP && K <= V, "token_logprobs: top_k ", K, " not in [0, ", MAX_TOP, "]");
-  TORCH_CHECK(ids.is_cuda() && ids.scalar_type() == at::kLong && ids.is_contiguous() && ids.numel() == logits.size(0),
-              "token_logprobs: one int64 id per row");
+// logits: [N, >= V] bf16 / fp16 / fp32, any row stride; only the first V columns are read, whatever the rest holds
+// (V = 0: all). ids: [N] int64 or int32 (less vocab_offset outside [0, V): log-probability -inf). Returns fp32 [N]
+// log-probability, entropy and log-sum-exp, the K best log-probabilities [N, K] and their ids.
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> logits_stats(
+    at::Tensor logits, int64_t V, at::Tensor ids, int64_t vocab_offset, int64_t K, at::Tensor status) {
+  // plain messages: putting numbers into them needs streams that this extension does not bring along
+  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2, "token_logprobs: logits must be [rows, vocabulary] on CUDA");
   const int64_t N = logits.size(0);
+  if (V == 0) V = logits.size(1);
+  TORCH_CHECK(V > 0 && V <= logits.size(1) && V < (int64_t(1) << 30),
+              "token_logprobs: valid_vocab is outside the logits' columns");
+  static_assert(MAX_TOP == 32, "the message names it");
+  TORCH_CHECK(K >= 0 && K <= MAX_TOP && K <= V, "token_logprobs: top_k must be 0 to 32 and at most the vocabulary");
+  TORCH_CHECK(ids.dim() == 1 && ids.numel() == N && ids.device() == logits.device() &&
+                  (ids.scalar_type() == at::kLong || ids.scalar_type() == at::kInt),
+              "token_logprobs: ids must be one int64 or int32 per row on the logits' device");
+  const auto dt = logits.scalar_type();
+  TORCH_CHECK(dt == at::kFloat || dt == at::kBFloat16 || dt == at::kHalf,
+              "token_logprobs: takes bf16, fp16 or fp32 on CUDA");
+  const c10::cuda::CUDAGuard guard(logits.device());
+  if (logits.stride(1) != 1 && logits.size(1) > 1) logits = logits.contiguous();
+  ids = ids.to(at::kLong).contiguous();
   auto stats = at::empty({3, N}, logits.options().dtype(at::kFloat));
-  auto top_vals = at::empty({N, K}, logits.options().dtype(at::kFloat));
+  auto top_vals = at::empty({N, K}, stats.options());
   auto top_ids = at::empty({N, K}, ids.options());
   int* st = status.data_ptr<int>();
   if (N > 0) {
-    switch (logits.scalar_type()) {
-      case at::kFloat:
-        launch<float>(logits, (int)V, ids, vocab_offset, (int)K, stats, top_vals, top_ids, st);
-        break;
-      case at::kBFloat16:
-        launch<__nv_bfloat16>(logits, (int)V, ids, vocab_offset, (int)K, stats, top_vals, top_ids, st);
-        break;
-      case at::kHalf:
-        launch<__half>(logits, (int)V, ids, vocab_offset, (int)K, stats, top_vals, top_ids, st);
-        break;
-      default:
-        TORCH_CHECK(false, "token_logprobs: dtype ", logits.scalar_type());
-    }
+    if (dt == at::kFloat) launch<float>(logits, (int)V, ids, vocab_offset, (int)K, stats, top_vals, top_ids, st);
+    else if (dt == at::kHalf) launch<__half>(logits, (int)V, ids, vocab_offset, (int)K, stats, top_vals, top_ids, st);
+    else launch<__nv_bfloat16>(logits, (int)V, ids, vocab_offset, (int)K, stats, top_vals, top_ids, st);
   }
-  return {stats, top_vals, top_ids};
+  return {stats.select(0, 0), stats.select(0, 1), stats.select(0, 2), top_vals, top_ids};
 }

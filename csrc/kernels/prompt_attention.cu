@@ -17,8 +17,10 @@
 // the two tiles at the exponentials (with one thread per row 4 % faster, with two a loss); heads of 64 with one tile
 // per CTA and two CTAs per SM (687 us against 650).
 #include <ATen/core/Tensor.h>
+#include <ATen/ops/empty.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAException.h>
+#include <c10/cuda/CUDAGuard.h>
 #include "../common.cuh"
 #include "../tma_host.h"
 #include <algorithm>
@@ -390,6 +392,11 @@ __global__ void __launch_bounds__(THREADS, 1)
     for (int i = 0; i < 6; ++i) issued[i] = 0;
     snb::fence_mbar_init();
   }
+  if (threadIdx.x == LOAD_WARP * 32) {
+    snb::prefetch_tmap(&tq);
+    snb::prefetch_tmap(&tk);
+    snb::prefetch_tmap(&tv);
+  }
   if (warp == MMA_WARP) {
     snb::tmem_alloc(tmem_slot, 512);
     snb::tmem_relinquish();
@@ -405,8 +412,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   if (warp == LOAD_WARP) {
     int nq = 0, nk = 0, nv = 0;
     bool ok = true;
-    // It alone works the items out (a few global reads and divisions) and hands them over one item ahead, before it
-    // waits for the ring.
+    // It alone works the items out (a few global reads and divisions) and hands them over one item ahead.
     auto publish = [&](int r, Item& it) {
       const bool have = next_item(p, r, it);
       if (!have) it.kb0 = it.kb1 = 0;
@@ -421,44 +427,48 @@ __global__ void __launch_bounds__(THREADS, 1)
       return have;
     };
     Item it, next;
+    int hk = 0;
+    auto load_k = [&](int kb) {
+      const int s = nk % C::NK;
+      if (!snb::mbar_wait_bounded(&k_empty[s], ((nk / C::NK) & 1) ^ 1, status, SNB_ERR_TIMEOUT_TMA)) return false;
+      snb::mbar_arrive_expect_tx(&k_full[s], C::KB);
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c)
+        snb::tma_load_2d(sK + s * C::KB + c * CHUNK, &tk, &k_full[s], hk * D + c * 64, it.first + kb * BKV);
+      ++nk;
+      return true;
+    };
+    auto load_v = [&](int kb) {
+      const int s = nv % C::NV;
+      if (!snb::mbar_wait_bounded(&v_empty[s], ((nv / C::NV) & 1) ^ 1, status, SNB_ERR_TIMEOUT_TMA)) return false;
+      snb::mbar_arrive_expect_tx(&v_full[s], C::VB);
+#pragma unroll
+      for (int c = 0; c < DV / 64; ++c)
+        snb::tma_load_2d(sV + s * C::VB + c * CHUNK, &tv, &v_full[s], hk * DV + c * 64, it.first + kb * BKV);
+      ++nv;
+      return true;
+    };
+    auto load_q = [&]() {
+      if (!snb::mbar_wait_bounded(q_empty, (nq & 1) ^ 1, status, SNB_ERR_TIMEOUT_TMA)) return false;
+      snb::mbar_arrive_expect_tx(q_full, 2 * C::QB);
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c)
+          snb::tma_load_2d(sQ + j * C::QB + c * CHUNK, &tq, q_full, (it.h0 + (p.pair_heads ? j : 0)) * D + c * 64,
+                           it.first + it.r0 + (p.pair_heads ? 0 : j * BQ));
+      ++nq;
+      return true;
+    };
     bool have = publish(0, it);
     for (int r = 0; ok && have; ++r, it = next) {
+      hk = it.h0 / G;
+      if (lane == 0) ok = load_k(it.kb0) && load_q();
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+      if (!ok) break;
       have = publish(r + 1, next);
-      if (lane == 0 && ok) {
-        const int hk = it.h0 / G;
-        auto load_k = [&](int kb) {
-          const int s = nk % C::NK;
-          if (!snb::mbar_wait_bounded(&k_empty[s], ((nk / C::NK) & 1) ^ 1, status, SNB_ERR_TIMEOUT_TMA)) return false;
-          snb::mbar_arrive_expect_tx(&k_full[s], C::KB);
-#pragma unroll
-          for (int c = 0; c < D / 64; ++c)
-            snb::tma_load_2d(sK + s * C::KB + c * CHUNK, &tk, &k_full[s], hk * D + c * 64, it.first + kb * BKV);
-          ++nk;
-          return true;
-        };
-        auto load_v = [&](int kb) {
-          const int s = nv % C::NV;
-          if (!snb::mbar_wait_bounded(&v_empty[s], ((nv / C::NV) & 1) ^ 1, status, SNB_ERR_TIMEOUT_TMA)) return false;
-          snb::mbar_arrive_expect_tx(&v_full[s], C::VB);
-#pragma unroll
-          for (int c = 0; c < DV / 64; ++c)
-            snb::tma_load_2d(sV + s * C::VB + c * CHUNK, &tv, &v_full[s], hk * DV + c * 64, it.first + kb * BKV);
-          ++nv;
-          return true;
-        };
-        ok = load_k(it.kb0) && snb::mbar_wait_bounded(q_empty, (nq & 1) ^ 1, status, SNB_ERR_TIMEOUT_TMA);
-        if (ok) {
-          snb::mbar_arrive_expect_tx(q_full, 2 * C::QB);
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int c = 0; c < D / 64; ++c)
-              snb::tma_load_2d(sQ + j * C::QB + c * CHUNK, &tq, q_full, (it.h0 + (p.pair_heads ? j : 0)) * D + c * 64,
-                               it.first + it.r0 + (p.pair_heads ? 0 : j * BQ));
-          ++nq;
-          for (int kb = it.kb0; ok && kb < it.kb1; ++kb) ok = load_v(kb) && (kb + 1 == it.kb1 || load_k(kb + 1));
-        }
-      }
+      if (lane == 0)
+        for (int kb = it.kb0; ok && kb < it.kb1; ++kb) ok = load_v(kb) && (kb + 1 == it.kb1 || load_k(kb + 1));
       ok = __shfl_sync(0xffffffffu, ok, 0);
     }
     if (lane == 0) issued[0] = nq, issued[1] = nk, issued[2] = nv;
@@ -819,39 +829,57 @@ void dispatch(const PromptParams& p, int64_t D, int64_t DV, int* status, cudaStr
   if (D == 64 && DV == 64) launch<T, 64, 64>(p, status, st);
   else if (D == 128 && DV == 128) launch<T, 128, 128>(p, status, st);
   else if (D == 192 && DV == 128) launch<T, 192, 128>(p, status, st);
-  else TORCH_CHECK(false, "prompt_attention: head dims ", D, " / ", DV, " (64 / 64, 128 / 128 or 192 / 128)");
+  else TORCH_CHECK(false, "prompt_attention: serves keys / values 64 / 64, 128 / 128 or 192 / 128 wide");
 }
 
-void check_rows(const at::Tensor& x, int64_t T, int64_t width, at::ScalarType dt, const char* name) {
-  TORCH_CHECK(x.is_cuda() && x.dim() == 2 && x.size(0) == T && x.size(1) == width && x.scalar_type() == dt,
-              "prompt_attention: ", name, " must be a CUDA matrix of ", T, " x ", width, " and the queries' type");
-  TORCH_CHECK(x.stride(1) == 1 && x.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0,
-              "prompt_attention: ", name, " needs contiguous rows on 16-byte boundaries");
+bool readable(const at::Tensor& x) {  // contiguous rows on 16-byte boundaries
+  return x.stride(1) == 1 && x.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
+}
+
+bool is_matrix(const at::Tensor& x, int64_t T, int64_t width, const at::Tensor& q) {
+  return x.dim() == 2 && x.size(0) == T && x.size(1) == width && x.scalar_type() == q.scalar_type() &&
+         x.device() == q.device();
 }
 
 }  // namespace
 
-// q [T, heads * D], k [T, kv_heads * D], v [T, kv_heads * DV], out [T, heads * DV]: bf16 or fp16, any row stride
-// that is a multiple of 8. indptr [B + 1] int32, ascending; rows outside every prompt are not written.
-void prompt_attention(at::Tensor out, at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor indptr,
-                      int64_t heads, int64_t kv_heads, int64_t D, int64_t DV, int64_t window, double sm_scale,
-                      std::optional<at::Tensor> sinks, at::Tensor status) {
-  const int64_t T = q.size(0), B = indptr.numel() - 1;
-  TORCH_CHECK(heads > 0 && kv_heads > 0 && heads % kv_heads == 0, "prompt_attention: ", heads, " heads over ",
-              kv_heads, " KV heads");
+// q [T, heads * D], k [T, kv_heads * D], v [T, kv_heads * DV]: bf16 or fp16 (rows that are not contiguous or not on
+// 16-byte boundaries are copied first); out [T, heads * DV] or none. indptr [B + 1] int32, ascending; rows outside
+// every prompt are not written.
+at::Tensor prompt_attention(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor indptr, int64_t heads,
+                            int64_t kv_heads, int64_t D, int64_t DV, int64_t window, double sm_scale,
+                            std::optional<at::Tensor> sinks, std::optional<at::Tensor> given, at::Tensor status) {
+  // the messages are plain text: putting numbers into them needs streams that this extension does not bring along
+  TORCH_CHECK(q.is_cuda() && q.dim() == 2, "prompt_attention: q must be a CUDA matrix");
+  TORCH_CHECK(heads > 0 && kv_heads > 0 && heads % kv_heads == 0,
+              "prompt_attention: the heads do not divide over the KV heads");
+  TORCH_CHECK(window >= 0 && sm_scale > 0,
+              "prompt_attention: the window must be 0 (off) or more, sm_scale must be positive");
   const auto dt = q.scalar_type();
-  check_rows(q, T, heads * D, dt, "q");
-  check_rows(k, T, kv_heads * D, dt, "k");
-  check_rows(v, T, kv_heads * DV, dt, "v");
-  check_rows(out, T, heads * DV, dt, "out");
-  TORCH_CHECK(indptr.is_cuda() && indptr.scalar_type() == at::kInt && indptr.is_contiguous() && B >= 0,
-              "prompt_attention: indptr must be a CUDA int32 vector");
+  TORCH_CHECK(dt == at::kBFloat16 || dt == at::kHalf, "prompt_attention: takes bf16 or fp16 on CUDA");
+  const int64_t T = q.size(0), B = indptr.numel() - 1;
+  TORCH_CHECK(is_matrix(q, T, heads * D, q), "prompt_attention: q must be [tokens, heads * head_dim]");
+  TORCH_CHECK(is_matrix(k, T, kv_heads * D, q),
+              "prompt_attention: k must be [tokens, KV heads * head_dim] of q's type and device");
+  TORCH_CHECK(is_matrix(v, T, kv_heads * DV, q),
+              "prompt_attention: v must be [tokens, KV heads * v_head_dim] of q's type and device");
+  TORCH_CHECK(indptr.dim() == 1 && B >= 0 && indptr.scalar_type() == at::kInt && indptr.device() == q.device(),
+              "prompt_attention: qo_indptr must be an int32 vector of prompt bounds on q's device");
   TORCH_CHECK(T < (int64_t(1) << 30), "prompt_attention: too many tokens");
   if (sinks)
-    TORCH_CHECK(sinks->is_cuda() && sinks->scalar_type() == at::kFloat && sinks->is_contiguous() &&
+    TORCH_CHECK(sinks->device() == q.device() && sinks->scalar_type() == at::kFloat && sinks->is_contiguous() &&
                     sinks->numel() == heads,
-                "prompt_attention: sinks must be one fp32 value per head");
-  if (T == 0 || B == 0) return;
+                "prompt_attention: sinks must be one fp32 value per head on q's device");
+  const c10::cuda::CUDAGuard guard(q.device());
+  at::Tensor out = given ? *given : at::empty({T, heads * DV}, q.options());
+  TORCH_CHECK(is_matrix(out, T, heads * DV, q),
+              "prompt_attention: out must be [tokens, heads * v_head_dim] of q's type and device");
+  TORCH_CHECK(T == 0 || readable(out), "prompt_attention: out needs contiguous rows on 16-byte boundaries");
+  if (T == 0 || B == 0) return out;
+  if (!readable(q)) q = q.contiguous();
+  if (!readable(k)) k = k.contiguous();
+  if (!readable(v)) v = v.contiguous();
+  indptr = indptr.contiguous();
   PromptParams p;
   p.q = q.data_ptr();
   p.k = k.data_ptr();
@@ -867,10 +895,10 @@ void prompt_attention(at::Tensor out, at::Tensor q, at::Tensor k, at::Tensor v, 
   p.B = (int)B;
   p.heads = (int)heads;
   p.kv_heads = (int)kv_heads;
-  p.window = (int)std::min<int64_t>(std::max<int64_t>(window, 0), T);
+  p.window = (int)std::min<int64_t>(window, T);
   p.scale = (float)(sm_scale * 1.4426950408889634);
   auto st = at::cuda::getCurrentCUDAStream();
   if (dt == at::kBFloat16) dispatch<__nv_bfloat16>(p, D, DV, status.data_ptr<int>(), st);
-  else if (dt == at::kHalf) dispatch<__half>(p, D, DV, status.data_ptr<int>(), st);
-  else TORCH_CHECK(false, "prompt_attention: dtype ", dt);
+  else dispatch<__half>(p, D, DV, status.data_ptr<int>(), st);
+  return out;
 }

@@ -44,7 +44,6 @@ class _CountingKernels:
 
     def __init__(self, mod):
         self._mod = mod
-        self._cache = {}
 
     def __getattr__(self, name):
         fn = getattr(self._mod, name)
@@ -61,11 +60,12 @@ class _CountingKernels:
                 _launches[0] += 2  # the product with its partial statistics, and their join
                 return fn(*a, **k)
         elif name in _HOST_ONLY:
-            return fn
+            call = fn
         else:
             def call(*a, **k):
                 _launches[0] += 1
                 return fn(*a, **k)
+        self.__dict__[name] = call  # found directly from now on
         return call
 
 
@@ -83,6 +83,17 @@ def kernels():
     if _counting is None:
         _counting = _CountingKernels(_C)
     return _counting
+
+
+def checked(op: str, name: str, *args):
+    """Runs kernel entry `name`, whose checks of its arguments say which operator they belong to: those become
+    ValueError."""
+    try:
+        return getattr(kernels(), name)(*args)
+    except RuntimeError as e:
+        if str(e).startswith(op + ":"):
+            raise ValueError(str(e).split("\n")[0]) from None
+        raise
 
 
 def runtime():

@@ -11,7 +11,7 @@ from typing import NamedTuple
 
 import torch
 
-from .._ext import kernels
+from .._ext import checked
 from .gemm import TiledWeight, _status_buf
 
 MAX_TOP = 32
@@ -63,55 +63,41 @@ def _check(rows: int, cols: int, ids: torch.Tensor, top_k: int, valid_vocab: int
     return V
 
 
-def _long(ids: torch.Tensor) -> torch.Tensor:
-    return ids if ids.dtype == torch.int64 and ids.is_contiguous() else ids.long().contiguous()
-
-
 def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, top_k: int = 0, vocab_offset: int = 0,
                    valid_vocab: int = 0) -> TokenLogprobs:
-    """`logits` [N, C] (bf16, fp16 or fp32; any row stride), `ids` [N]; see TokenLogprobs."""
+    """`logits` [N, C] (bf16, fp16 or fp32 on CUDA; any row stride), `ids` [N]; see TokenLogprobs."""
+    if logits.is_cuda:  # the kernel's entry checks its arguments (ValueError)
+        return TokenLogprobs(*checked("token_logprobs", "logits_stats", logits, valid_vocab, ids, vocab_offset, top_k,
+                                      _status_buf(logits.device)))
     if logits.dim() != 2:
         raise ValueError(f"logits must be [rows, vocabulary], got {tuple(logits.shape)}")
     V = _check(logits.shape[0], logits.shape[1], ids, top_k, valid_vocab)
-    if not logits.is_cuda:
-        return token_logprobs_ref(logits, ids, top_k, vocab_offset, V)
-    if logits.dtype not in (torch.bfloat16, torch.float16, torch.float32):
-        raise ValueError(f"token_logprobs takes bf16, fp16 or fp32 on CUDA, got {logits.dtype}")
-    if logits.stride(1) != 1 and logits.shape[1] > 1:
-        logits = logits.contiguous()
-    stats, tl, ti = kernels().logits_stats(logits, V, _long(ids), vocab_offset, top_k, _status_buf(logits.device))
-    return TokenLogprobs(*stats.unbind(0), tl, ti)
+    return token_logprobs_ref(logits, ids, top_k, vocab_offset, V)
 
 
 def head_logprobs(hidden: torch.Tensor, weight, ids: torch.Tensor, vocab_offset: int = 0,
                   valid_vocab: int = 0) -> TokenLogprobs:
     """The same of the logits `hidden @ weight.T`, which are kept in fp32 (never rounded, never stored). `hidden`
-    [N, H] bf16 or fp16, `weight` [V, H] of the same type (a tensor or a TiledWeight), H a multiple of 8. Gives no
-    alternatives: those need the logits (`token_logprobs`)."""
+    [N, H] bf16 or fp16 on CUDA, `weight` [V, H] of the same type (a tensor or a TiledWeight), H a multiple of 8. Gives
+    no alternatives: those need the logits (`token_logprobs`)."""
+    tiled, F = False, 0
+    if isinstance(weight, TiledWeight):
+        if hidden.dim() != 2 or hidden.shape[1] != weight.K:
+            raise ValueError(f"hidden {tuple(hidden.shape)} does not fit the weight {tuple(weight.shape)}")
+        tiled, F = weight.rowmajor is None and hidden.is_cuda, weight.F
+        weight = weight.data if tiled else weight.rowmajor if weight.rowmajor is not None else weight.untiled()
+    if hidden.is_cuda:  # the kernel's entry checks its arguments (ValueError)
+        lp, ent, lse = checked("head_logprobs", "head_stats", hidden, weight, F, tiled, valid_vocab, ids, vocab_offset,
+                               _status_buf(hidden.device))
+        return TokenLogprobs(lp, ent, lse, lp.new_empty(lp.shape[0], 0),
+                             ids.new_empty(lp.shape[0], 0, dtype=torch.int64))
     if hidden.dim() != 2 or hidden.shape[1] != weight.shape[1]:
         raise ValueError(f"hidden {tuple(hidden.shape)} does not fit the weight {tuple(weight.shape)}")
     if hidden.dtype != weight.dtype:
         raise ValueError(f"hidden is {hidden.dtype}, the weight {weight.dtype}")
     V = _check(hidden.shape[0], weight.shape[0], ids, 0, valid_vocab)
-    if not hidden.is_cuda:
-        w = weight.untiled() if isinstance(weight, TiledWeight) else weight
-        wide = torch.float64 if hidden.dtype == torch.float64 else torch.float32
-        return token_logprobs_ref(hidden.to(wide) @ w[:V].to(wide).t(), ids, 0, vocab_offset, V)
-    if hidden.dtype not in (torch.bfloat16, torch.float16):
-        raise ValueError(f"head_logprobs takes bf16 or fp16 on CUDA, got {hidden.dtype}")
-    N, H = hidden.shape
-    if H % 8:
-        raise ValueError(f"head_logprobs needs a hidden size that is a multiple of 8, got {H}")
-    tiled = False
-    if isinstance(weight, TiledWeight):
-        tiled = weight.rowmajor is None
-        weight = weight.data if tiled else weight.rowmajor
-    if hidden.stride(1) != 1 or hidden.stride(0) % 8 or hidden.data_ptr() % 16:
-        hidden = hidden.contiguous()
-    if not tiled and (weight.stride(1) != 1 or weight.stride(0) % 8 or weight.data_ptr() % 16):
-        weight = weight.contiguous()
-    stats = kernels().head_stats(hidden, weight, V, tiled, _long(ids), vocab_offset, _status_buf(hidden.device))
-    return TokenLogprobs(*stats.unbind(0), stats.new_empty(N, 0), ids.new_empty(N, 0, dtype=torch.int64))
+    wide = torch.float64 if hidden.dtype == torch.float64 else torch.float32
+    return token_logprobs_ref(hidden.to(wide) @ weight[:V].to(wide).t(), ids, 0, vocab_offset, V)
 
 
 def merge_shards(shards) -> TokenLogprobs:

@@ -8,12 +8,9 @@ from typing import Optional
 
 import torch
 
-from .._ext import kernels
+from .._ext import checked
 from .attention import _attend_ref
 from .gemm import _status_buf
-
-# (key width, value width) the kernel serves
-HEAD_DIMS = ((64, 64), (128, 128), (192, 128))
 
 
 def prompt_attention_ref(q, k, v, qo_indptr, num_q_heads, num_kv_heads, head_dim, v_head_dim=None, window=0,
@@ -34,23 +31,20 @@ def prompt_attention_ref(q, k, v, qo_indptr, num_q_heads, num_kv_heads, head_dim
     return out.reshape(T, num_q_heads * v_head_dim)
 
 
-def _rows(x: torch.Tensor) -> torch.Tensor:
-    """x with rows the kernel can read: contiguous, on 16-byte boundaries."""
-    if x.stride(1) != 1 or x.stride(0) % 8 or x.data_ptr() % 16:
-        return x.contiguous()
-    return x
-
-
 def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, qo_indptr: torch.Tensor, num_q_heads: int,
                      num_kv_heads: int, head_dim: int, v_head_dim: Optional[int] = None, window: int = 0,
                      sm_scale: Optional[float] = None, sinks: Optional[torch.Tensor] = None,
                      out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Tokens [qo_indptr[b], qo_indptr[b + 1]) are prompt b; every token attends to itself and the tokens before it
     in its prompt (the last `window` of them where window > 0). q [T, num_q_heads * head_dim], k and v [T,
-    num_kv_heads * width]: bf16 or fp16 on CUDA, views with a row stride (columns of a fused projection) included.
+    num_kv_heads * width]: bf16 or fp16 and widths of 64, 128 or 192 (values 128) on CUDA; views with a row stride
+    (columns of a fused projection) are read in place.
     Returns [T, num_q_heads * v_head_dim]; rows outside every prompt are left as they are."""
     v_head_dim = head_dim if v_head_dim is None else v_head_dim
     sm_scale = head_dim ** -0.5 if sm_scale is None else sm_scale
+    if q.is_cuda:  # the kernel's entry checks its arguments (ValueError)
+        return checked("prompt_attention", "prompt_attention", q, k, v, qo_indptr, num_q_heads, num_kv_heads, head_dim,
+                       v_head_dim, window, sm_scale, sinks, out, _status_buf(q.device))
     if num_kv_heads <= 0 or num_q_heads % num_kv_heads:
         raise ValueError(f"{num_q_heads} heads do not divide over {num_kv_heads} KV heads")
     T = q.shape[0]
@@ -66,19 +60,9 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, qo_indpt
         raise ValueError(f"{sinks.numel()} sinks for {num_q_heads} heads")
     if out is not None and tuple(out.shape) != (T, num_q_heads * v_head_dim):
         raise ValueError(f"out is {tuple(out.shape)}, expected {(T, num_q_heads * v_head_dim)}")
-    if not q.is_cuda:
-        r = prompt_attention_ref(q, k, v, qo_indptr, num_q_heads, num_kv_heads, head_dim, v_head_dim, window,
-                                 sm_scale, sinks).to(q.dtype)
-        if out is not None:
-            out.copy_(r)
-            return out
-        return r
-    if q.dtype not in (torch.bfloat16, torch.float16):
-        raise ValueError(f"prompt_attention takes bf16 or fp16 on CUDA, got {q.dtype}")
-    if (head_dim, v_head_dim) not in HEAD_DIMS:
-        raise ValueError(f"prompt_attention serves head dims {HEAD_DIMS} on CUDA, got {(head_dim, v_head_dim)}")
-    if out is None:
-        out = torch.empty(T, num_q_heads * v_head_dim, dtype=q.dtype, device=q.device)
-    kernels().prompt_attention(out, _rows(q), _rows(k), _rows(v), qo_indptr, num_q_heads, num_kv_heads, head_dim,
-                               v_head_dim, window, sm_scale, sinks, _status_buf(q.device))
-    return out
+    r = prompt_attention_ref(q, k, v, qo_indptr, num_q_heads, num_kv_heads, head_dim, v_head_dim, window, sm_scale,
+                             sinks).to(q.dtype)
+    if out is not None:
+        out.copy_(r)
+        return out
+    return r

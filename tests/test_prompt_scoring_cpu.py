@@ -228,3 +228,17 @@ def test_sharded_scores_equal_tp1():
             if "input_top_logprobs" in x:
                 assert [[t for _, t in r] for r in x["input_top_logprobs"][1:]] == \
                        [[t for _, t in r] for r in y["input_top_logprobs"][1:]]
+
+
+def test_kernel_entries_refuse_without_a_crash():
+    """The compiled entries' own checks come back as exceptions (ValueError through the operators)."""
+    from sglang_neuron_b200 import _ext
+    if not _ext.available():
+        pytest.skip("extension not built")
+    x = torch.zeros(4, 8, dtype=torch.bfloat16)
+    ids, st, ip = torch.zeros(4, dtype=torch.long), torch.zeros(4, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    for op, name, args in [("prompt_attention", "prompt_attention", (x, x, x, ip, 3, 2, 4, 4, 0, 0.1, None, None, st)),
+                           ("token_logprobs", "logits_stats", (x, 99, ids, 0, 0, st)),
+                           ("head_logprobs", "head_stats", (x, x, 0, False, 0, ids, 0, st))]:
+        with pytest.raises(ValueError, match=op):
+            _ext.checked(op, name, *args)
