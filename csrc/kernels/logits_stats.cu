@@ -10,7 +10,8 @@
 // bytes per load and keeps the maximum of every two loads (a segment), which the running reference needs anyway. The K-th
 // best of 32 groups' maxima is a lower bound of the K-th best entry, so afterwards only the segments whose
 // maximum reaches it are read again (they are in L2) and sorted in by (value, ~id) keys: about K segments for
-// ordinary rows, all of them for a constant row.
+// ordinary rows, all of them for a constant row. The CTAs of a cluster exchange the groups' maxima, so that a row has
+// these K segments once, not once per CTA (64 x 201088 fp32 with twenty: 26.3 us without the exchange, 20.5 with it).
 //
 // Bound: the logits' bytes at DRAM rate. A bf16 row at that rate brings 12 logits a clock and SM, so a logit has one
 // exponential (of 16 a clock) and few issue slots: two values go through each fp32 instruction (f32x2), y is taken in
@@ -18,10 +19,10 @@
 // -6e4) keeps 0 * y finite where a logit is masked; a CTA whose every logit lies down there reads its part once more
 // on an exact path.
 // The row comes through a ring of three 16 KB bulk copies that one thread keeps full.
-// Measured on a B200: 4096 x 151936 bf16 without alternatives 235 us (5.3 TB/s), with five 262 us, with twenty 305 us
+// Measured on a B200: 4096 x 151936 bf16 without alternatives 234 us (5.3 TB/s), with five 254 us, with twenty 301 us
 // (choosing them takes a CTA some 5 us after its row); 1000 x 201088 fp32 with five 135 us (6.0 TB/s); 64 x 201088 fp32
-// without alternatives 14.5 us, with twenty 26 us; a single bf16 row with five 9 us, without 5 us. Tried and slower:
-// CTAs that stay and load the next row's first stages while they choose (280 us with five); the bound from 64 groups.
+// without alternatives 14.2 us, with twenty 20.5 to 21.8 us. Tried and slower: CTAs that stay and load the next row's
+// first stages while they choose (280 us with five); the bound from 64 groups.
 // Split: one CTA per row, four resident per SM; fewer rows than that put a cluster of 2 to 8 CTAs on each row, whose
 // partial results the first CTA joins through distributed shared memory.
 #include <ATen/core/Tensor.h>
@@ -209,11 +210,14 @@ __global__ void __launch_bounds__(THREADS, 4)
   __shared__ float row_c, row_lg;
   __shared__ Stats cta_stats[MAX_CLUSTER];
   __shared__ uint64_t cand[WARPS * MAX_TOP];
+  uint32_t* groups = reinterpret_cast<uint32_t*>(cand);  // before it: the groups' maxima of every CTA of the cluster
+  static_assert(sizeof(cand) >= MAX_CLUSTER * 32 * 4, "");
   __shared__ uint64_t lists[MAX_CLUSTER * MAX_TOP];  // filled by every CTA of the cluster in the first one's memory
   __shared__ int cand_n, best_n[MAX_CLUSTER];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int C = gridDim.x, rank = blockIdx.x;  // the cluster spans the grid's x axis
+  const uint32_t dst_rank = 0;
   const int64_t row = blockIdx.y;
   if (threadIdx.x == 0) {
     if (TOP) cand_n = 0;
@@ -372,12 +376,46 @@ __global__ void __launch_bounds__(THREADS, 4)
   }
   __syncthreads();
 
+  // this CTA's sums into the first CTA's shared memory, its groups' maxima into every CTA's
+  if (C > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+  if (warp == WARPS) {  // the warp that has the least to do
+    Stats a;
+    a.c = most;
+    a.s = lane_sum<WARPS>(lane < WARPS ? warp_s[lane] : 0.f);
+    a.t = lane_sum<WARPS>(lane < WARPS ? warp_t[lane] : 0.f);
+    if (lane == 0) {
+      const uint32_t at = snb::mapa_shared(snb::smem_u32(&cta_stats[rank]), dst_rank);
+      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(a.c) : "memory");
+      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at + 4), "f"(a.s) : "memory");
+      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at + 8), "f"(a.t) : "memory");
+    }
+    __syncwarp();
+  }
+  // the maximum of a group: the threads of one lane number
+  uint32_t g = 0;
   if constexpr (TOP) {
-    // a lower bound of the K-th best entry: the K-th largest of 32 groups' maxima, a group being the threads of one
-    // lane number (0 when fewer than K groups hold any entry); every warp finds it for itself
-    uint32_t g = 0;
 #pragma unroll
     for (int i = 0; i < WARPS; ++i) g = max(g, best_keys[i * 32 + lane]);
+    if (C > 1 && warp < C)
+      asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(
+                       snb::mapa_shared(snb::smem_u32(&groups[rank * 32 + lane]), warp)),
+                   "r"(g)
+                   : "memory");
+  }
+  if (C > 1) {
+    snb::cluster_sync();
+    if (!TOP && rank != 0) return;
+  } else if (!TOP) {
+    __syncthreads();
+  }
+
+  if constexpr (TOP) {
+    // a lower bound of the row's K-th best entry: the K-th largest of 32 groups' maxima, over the whole cluster (0 when
+    // fewer than K groups hold any entry); every warp finds it for itself
+    if (C > 1) {
+      for (int i = 0; i < C; ++i) g = max(g, groups[i * 32 + lane]);
+      __syncthreads();
+    }
     int above = 0;
 #pragma unroll
     for (int i = 0; i < 32; ++i) above += __shfl_sync(0xffffffffu, g, i) > g;
@@ -450,28 +488,8 @@ __global__ void __launch_bounds__(THREADS, 4)
     if (lane == 0 && vm) base = atomicAdd(&cand_n, __popc(vm));
     base = __shfl_sync(0xffffffffu, base, 0);
     if (valid) cand[base + lane] = list;
-  }
-  __syncthreads();
-
-  // this CTA's result, into the first CTA's shared memory
-  const uint32_t dst_rank = 0;
-  if (C > 1) {
-    __syncwarp();
-    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
-  }
-  if (warp == WARPS) {  // the warp that has the least to do
-    Stats a;
-    a.c = most;
-    a.s = lane_sum<WARPS>(lane < WARPS ? warp_s[lane] : 0.f);
-    a.t = lane_sum<WARPS>(lane < WARPS ? warp_t[lane] : 0.f);
-    if (lane == 0) {
-      const uint32_t at = snb::mapa_shared(snb::smem_u32(&cta_stats[rank]), dst_rank);
-      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(a.c) : "memory");
-      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at + 4), "f"(a.s) : "memory");
-      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at + 8), "f"(a.t) : "memory");
-    }
-  }
-  if constexpr (TOP) {
+    __syncthreads();
+    // the CTA's best K of its warps' lists, into the first CTA's shared memory
     const int n = cand_n;  // at most WARPS * MAX_TOP
     for (int i = threadIdx.x; i < n; i += THREADS) {
       const uint64_t k = cand[i];
@@ -487,13 +505,13 @@ __global__ void __launch_bounds__(THREADS, 4)
       const uint32_t at = snb::mapa_shared(snb::smem_u32(&best_n[rank]), dst_rank);
       asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(min(n, K)) : "memory");
     }
-  }
-  if (C > 1) {
-    __syncwarp();
-    snb::cluster_sync();
-    if (rank != 0) return;
-  } else {
-    __syncthreads();
+    if (C > 1) {
+      __syncwarp();
+      snb::cluster_sync();
+      if (rank != 0) return;
+    } else {
+      __syncthreads();
+    }
   }
 
   if (warp == WARPS) {
@@ -517,7 +535,7 @@ __global__ void __launch_bounds__(THREADS, 4)
     }
   }
   if constexpr (TOP) {
-    // a merged list's places: the lists are sorted and their keys differ, so an entry's place is the sum of its ranks
+    // the lists' entries differ: an entry's place is how many of all come before it
     const int i = threadIdx.x, r = i / MAX_TOP, p = i % MAX_TOP;
     uint64_t k = 0;
     int at = K;
@@ -525,14 +543,9 @@ __global__ void __launch_bounds__(THREADS, 4)
       k = lists[i];
       at = p;
       for (int q = 0; q < C; ++q) {
-        if (q == r) continue;
-        int lo = 0, hi = best_n[q];  // how many of list q come before
-        while (lo < hi) {
-          const int mid = (lo + hi) / 2;
-          if (lists[q * MAX_TOP + mid] > k) lo = mid + 1;
-          else hi = mid;
-        }
-        at += lo;
+        const int n = q == r ? 0 : best_n[q];
+#pragma unroll 4
+        for (int j = 0; j < n; ++j) at += lists[q * MAX_TOP + j] > k;
       }
     }
     __syncthreads();
