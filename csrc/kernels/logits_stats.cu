@@ -26,8 +26,8 @@
 // Split: one CTA per row, four resident per SM; fewer rows than that put a cluster of 2 to 8 CTAs on each row, whose
 // partial results the first CTA joins through distributed shared memory.
 #include <ATen/core/Tensor.h>
-#include <ATen/ops/empty.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
 #include "../common.cuh"
@@ -558,7 +558,8 @@ __global__ void __launch_bounds__(THREADS, 4)
 
 template <typename T>
 void launch(const at::Tensor& logits, int V, const at::Tensor& ids, int64_t vocab_offset, int K,
-            at::Tensor& stats, at::Tensor& top_vals, at::Tensor& top_ids, int* status) {
+            at::Tensor& logprobs, at::Tensor& entropy, at::Tensor& lse, at::Tensor& top_vals, at::Tensor& top_ids,
+            int* status) {
   const int64_t rows = logits.size(0);
   const auto* prop = at::cuda::getCurrentDeviceProperties();
   auto st = at::cuda::getCurrentCUDAStream();
@@ -587,13 +588,13 @@ void launch(const at::Tensor& logits, int V, const at::Tensor& ids, int64_t voca
     cfg.numAttrs = snb::pdl_enabled() ? 2 : 1;
     const T* x = reinterpret_cast<const T*>(logits.data_ptr()) + r0 * logits.stride(0);
     const int64_t* id = ids.data_ptr<int64_t>() + r0;
-    float* out = stats.data_ptr<float>() + r0;
     float* tv = K > 0 ? top_vals.data_ptr<float>() + r0 * K : nullptr;
     int64_t* ti = K > 0 ? top_ids.data_ptr<int64_t>() + r0 * K : nullptr;
     auto kern = K > 0 ? logits_stats_kernel<T, true> : logits_stats_kernel<T, false>;
     C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, x, logits.stride(0), V, id, vocab_offset, K,
-                                      out, out + rows, out + 2 * rows, tv, ti, status));
+                                      logprobs.data_ptr<float>() + r0, entropy.data_ptr<float>() + r0,
+                                      lse.data_ptr<float>() + r0, tv, ti, status));
   }
 }
 
@@ -620,15 +621,21 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> logits_st
               "token_logprobs: takes bf16, fp16 or fp32 on CUDA");
   const c10::cuda::CUDAGuard guard(logits.device());
   if (logits.stride(1) != 1 && logits.size(1) > 1) logits = logits.contiguous();
-  ids = ids.to(at::kLong).contiguous();
-  auto stats = at::empty({3, N}, logits.options().dtype(at::kFloat));
-  auto top_vals = at::empty({N, K}, stats.options());
-  auto top_ids = at::empty({N, K}, ids.options());
+  if (ids.scalar_type() != at::kLong) ids = ids.to(at::kLong);
+  ids = ids.contiguous();
+  auto make = [&](at::IntArrayRef size, at::ScalarType type) {
+    return at::Tensor(at::detail::empty_cuda(size, type, logits.device(), std::nullopt));
+  };
+  auto logprobs = make({N}, at::kFloat), entropy = make({N}, at::kFloat), lse = make({N}, at::kFloat);
+  auto top_vals = make({N, K}, at::kFloat), top_ids = make({N, K}, at::kLong);
   int* st = status.data_ptr<int>();
   if (N > 0) {
-    if (dt == at::kFloat) launch<float>(logits, (int)V, ids, vocab_offset, (int)K, stats, top_vals, top_ids, st);
-    else if (dt == at::kHalf) launch<__half>(logits, (int)V, ids, vocab_offset, (int)K, stats, top_vals, top_ids, st);
-    else launch<__nv_bfloat16>(logits, (int)V, ids, vocab_offset, (int)K, stats, top_vals, top_ids, st);
+    auto run = [&](auto kind) {
+      launch<decltype(kind)>(logits, (int)V, ids, vocab_offset, (int)K, logprobs, entropy, lse, top_vals, top_ids, st);
+    };
+    if (dt == at::kFloat) run(float());
+    else if (dt == at::kHalf) run(__half());
+    else run(__nv_bfloat16());
   }
-  return {stats.select(0, 0), stats.select(0, 1), stats.select(0, 2), top_vals, top_ids};
+  return {logprobs, entropy, lse, top_vals, top_ids};
 }
