@@ -349,8 +349,8 @@ SNB_DEVICE bool next_item(const PromptParams& p, int r, Item& it) {
 template <typename T, int D, int DV>
 __global__ void __launch_bounds__(THREADS, 1)
     prompt_attention_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
-                            const __grid_constant__ CUtensorMap tv, const __grid_constant__ PromptParams p,
-                            int* status) {
+                            const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap tq32,
+                            const __grid_constant__ PromptParams p, int* status) {
   using C = Cfg<D, DV>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -374,6 +374,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   int* taken = issued + 3;                              // and waited for
   float* sX = reinterpret_cast<float*>(taken + 3);      // [2][128] what the two halves of a row exchange
   Item* sItem = reinterpret_cast<Item*>(sX + 2 * BQ);   // [2]
+  float* sSink = reinterpret_cast<float*>(sItem + 2);   // [4][2] the sinks of an item's two heads
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -394,6 +395,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
   if (threadIdx.x == LOAD_WARP * 32) {
     snb::prefetch_tmap(&tq);
+    snb::prefetch_tmap(&tq32);
     snb::prefetch_tmap(&tk);
     snb::prefetch_tmap(&tv);
   }
@@ -417,9 +419,18 @@ __global__ void __launch_bounds__(THREADS, 1)
       const bool have = next_item(p, r, it);
       if (!have) it.kb0 = it.kb1 = 0;
       if (lane == 0) {
+        float sink[2] = {0.f, 0.f};
+        if (have && p.sinks != nullptr) {
+          sink[0] = __ldg(p.sinks + it.h0);
+          sink[1] = __ldg(p.sinks + it.h0 + (p.pair_heads ? 1 : 0));
+        }
         ok = snb::mbar_wait_bounded(&i_empty[r & 1], ((r >> 1) & 1) ^ 1, status, SNB_ERR_TIMEOUT_TMA);
         if (ok) {
           sItem[r & 1] = it;
+          // read at the item's end, when the slot of the item itself may be taken: item r - 4 is over by now, since
+          // every softmax warp has taken item r - 2
+          sSink[(r & 3) * 2] = sink[0];
+          sSink[(r & 3) * 2 + 1] = sink[1];
           snb::mbar_arrive(&i_full[r & 1]);
         }
       }
@@ -451,12 +462,18 @@ __global__ void __launch_bounds__(THREADS, 1)
     auto load_q = [&]() {
       if (!snb::mbar_wait_bounded(q_empty, (nq & 1) ^ 1, status, SNB_ERR_TIMEOUT_TMA)) return false;
       snb::mbar_arrive_expect_tx(q_full, 2 * C::QB);
+      // The second tile's quarters of 32 rows lie in the opposite order: a quarter belongs to one scheduler's warps, and
+      // where a mask cuts blocks (the diagonal, a window) its rows leave some quarters whole and some empty. Four
+      // prompts near 1024 tokens, 64 heads of 64, window 128: 54.8 us with both tiles in order, 50.8 us like this.
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int c = 0; c < D / 64; ++c) {
+        snb::tma_load_2d(sQ + c * CHUNK, &tq, q_full, it.h0 * D + c * 64, it.first + it.r0);
 #pragma unroll
-        for (int c = 0; c < D / 64; ++c)
-          snb::tma_load_2d(sQ + j * C::QB + c * CHUNK, &tq, q_full, (it.h0 + (p.pair_heads ? j : 0)) * D + c * 64,
-                           it.first + it.r0 + (p.pair_heads ? 0 : j * BQ));
+        for (int i = 0; i < 4; ++i)
+          snb::tma_load_2d(sQ + C::QB + c * CHUNK + (3 - i) * (CHUNK / 4), &tq32, q_full,
+                           (it.h0 + (p.pair_heads ? 1 : 0)) * D + c * 64,
+                           it.first + it.r0 + (p.pair_heads ? 0 : BQ) + i * 32);
+      }
       ++nq;
       return true;
     };
@@ -565,8 +582,8 @@ __global__ void __launch_bounds__(THREADS, 1)
     const int j = warp >> 3, h = (warp >> 2) & 1, bar = 1 + j * 4 + (warp & 3);
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_at = tmem + j * 128 + h * 64 + lanes, o_at = tmem + 256 + j * DV + h * (DV / 2) + lanes;
-    const int row = (warp & 3) * 32 + lane;
-    float* x = sX + j * BQ + row;
+    const int quarter = (j == 0 ? warp & 3 : 3 - (warp & 3)) * 32;  // its first row, see load_q
+    float* x = sX + j * BQ + (warp & 3) * 32 + lane;
     int ns = 0;  // blocks done by this tile, over all items
     bool ok = true;
     constexpr bool NARROW = std::is_same<T, __half>::value;
@@ -597,8 +614,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (it.kb0 == it.kb1) break;
       const int head = it.h0 + (p.pair_heads ? j : 0);
       const int r0 = it.r0 + (p.pair_heads ? 0 : j * BQ);
-      const int rel = r0 + row;  // this thread's query, counted from the prompt's first token
-      const int rw = r0 + (warp & 3) * 32;  // this warp's first query
+      const int rel = r0 + quarter + lane;  // this thread's query, counted from the prompt's first token
+      const int rw = r0 + quarter;  // this warp's first query
       const int lo = p.window > 0 ? rel - p.window + 1 : 0;
       float m = -INFINITY, l = 0.f;  // the reference, in log2 units; the weights' sum over this thread's keys
       for (int kb = it.kb0; kb < it.kb1; ++kb, ++ns) {
@@ -741,7 +758,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       l = exchange(l, [](float a, float b) { return a + b; });
       // NaN if the sum over the keys left its range or an output is not finite
       float zero = l > 0x1p-100f && l < 0x1p100f ? 0.f : NAN;
-      if (p.sinks != nullptr) l += ex2(p.sinks[head] * LOG2E - (m == -INFINITY ? 0.f : m));
+      if (p.sinks != nullptr) l += ex2(sSink[(r & 3) * 2 + j] * LOG2E - (m == -INFINITY ? 0.f : m));
       const float inv = m == -INFINITY ? 0.f : 1.f / l;  // only scores of -inf: nothing but the sink has weight
       const bool store = rel < it.len;
       const int t = it.first + rel;
@@ -781,7 +798,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         while (again) {
           const int src = __ffs(again) - 1;
           again &= again - 1;
-          attend_row<T, D, DV>(p, it.first, it.first + r0 + (warp & 3) * 32 + src, head);
+          attend_row<T, D, DV>(p, it.first, it.first + r0 + quarter + src, head);
         }
       }
     }
@@ -804,11 +821,11 @@ void launch(PromptParams p, int* status, cudaStream_t st) {
   using C = Cfg<D, DV>;
   constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
   const auto dt = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  auto map = [&](const void* base, int64_t width, int64_t stride) {
-    return snb_host::make_tmap_2d(base, dt, width, p.T, stride * 2, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+  auto map = [&](const void* base, int64_t width, int64_t stride, int rows = 128) {
+    return snb_host::make_tmap_2d(base, dt, width, p.T, stride * 2, 64, rows, CU_TENSOR_MAP_SWIZZLE_128B);
   };
   const CUtensorMap tq = map(p.q, (int64_t)p.heads * D, p.qs), tk = map(p.k, (int64_t)p.kv_heads * D, p.ks),
-                    tv = map(p.v, (int64_t)p.kv_heads * DV, p.vs);
+                    tv = map(p.v, (int64_t)p.kv_heads * DV, p.vs), tq32 = map(p.q, (int64_t)p.heads * D, p.qs, 32);
   p.idesc = bf16 ? 1u << 7 | 1u << 10 : 0u;
   p.pair_heads = (p.heads / p.kv_heads) % 2 == 0;
   p.pairs = p.pair_heads ? p.heads / 2 : p.heads;
@@ -820,8 +837,8 @@ void launch(PromptParams p, int* status, cudaStream_t st) {
   auto kern = prompt_attention_kernel<T, D, DV>;
   C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
   const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
-  C10_CUDA_CHECK(snb::launch_pdl(kern, dim3(std::min(p.items, sms)), dim3(THREADS), C::SMEM, st, tq, tk, tv, p,
-                                 status));
+  C10_CUDA_CHECK(snb::launch_pdl(kern, dim3(std::min(p.items, sms)), dim3(THREADS), C::SMEM, st, tq, tk, tv, tq32,
+                                 p, status));
 }
 
 template <typename T>
