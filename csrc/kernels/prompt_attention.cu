@@ -301,49 +301,55 @@ struct Item {
   int kb0, kb1;    // key blocks [kb0, kb1), counted from `first`; none: the list has ended
 };
 
-// Item w of the list (tile, head pair): the prompts in order, each prompt's tiles from its last one down. Called by
-// whole warps. False past the end.
-SNB_DEVICE bool decode_item(const PromptParams& p, int w, Item& it) {
+// How far the list has been counted: a CTA's items ascend, so it goes over the prompts' bounds once.
+struct Cursor {
+  int phase = 0, b0 = 0, before = 0;
+};
+
+// Item w of the list (tile, head pair): the prompts in order, each prompt's tiles from its last one down to the second,
+// then the first tiles of all prompts, which see the fewest keys and even out the end. Called by whole warps with
+// ascending w. False past the end.
+SNB_DEVICE bool decode_item(const PromptParams& p, int w, Cursor& at, Item& it) {
   const int lane = threadIdx.x & 31;
   const int rows = p.pair_heads ? BQ : 2 * BQ;
-  int idx = w / p.pairs;
-  const int pair = w % p.pairs;
-  for (int b0 = 0; b0 < p.B; b0 += 32) {
-    const int b = b0 + lane;
-    int a = 0, n = 0;
-    if (b < p.B) {
-      a = seq_bound(p, b);
-      n = max(0, seq_bound(p, b + 1) - a);
-    }
-    const int nt = (n + rows - 1) / rows;
-    int incl = nt;
+  const int idx = w / p.pairs, pair = w % p.pairs;
+  for (; at.phase < 2; ++at.phase, at.b0 = 0)
+    for (; at.b0 < p.B; at.b0 += 32) {
+      const int b = at.b0 + lane;
+      int a = 0, n = 0;
+      if (b < p.B) {
+        a = seq_bound(p, b);
+        n = max(0, seq_bound(p, b + 1) - a);
+      }
+      const int nt = (n + rows - 1) / rows;
+      int incl = at.phase == 0 ? max(nt - 1, 0) : min(nt, 1);
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int up = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += up;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += up;
+      }
+      const unsigned in = __ballot_sync(0xffffffffu, incl > idx - at.before);
+      if (in) {
+        const int src = __ffs(in) - 1;
+        it.first = __shfl_sync(0xffffffffu, a, src);
+        it.len = __shfl_sync(0xffffffffu, n, src);
+        it.r0 = at.phase == 0 ? (__shfl_sync(0xffffffffu, incl, src) - (idx - at.before)) * rows : 0;
+        it.h0 = p.pair_heads ? pair * 2 : pair;
+        it.kb1 = (min(it.len, it.r0 + rows) + BKV - 1) / BKV;
+        it.kb0 = p.window > 0 ? max(0, it.r0 - p.window + 1) / BKV : 0;
+        return true;
+      }
+      at.before += __shfl_sync(0xffffffffu, incl, 31);
     }
-    const unsigned in = __ballot_sync(0xffffffffu, incl > idx);
-    if (in) {
-      const int src = __ffs(in) - 1;
-      it.first = __shfl_sync(0xffffffffu, a, src);
-      it.len = __shfl_sync(0xffffffffu, n, src);
-      it.r0 = (__shfl_sync(0xffffffffu, incl, src) - 1 - idx) * rows;
-      it.h0 = p.pair_heads ? pair * 2 : pair;
-      it.kb1 = (min(it.len, it.r0 + rows) + BKV - 1) / BKV;
-      it.kb0 = p.window > 0 ? max(0, it.r0 - p.window + 1) / BKV : 0;
-      return true;
-    }
-    idx -= __shfl_sync(0xffffffffu, incl, 31);
-  }
   return false;
 }
 
-// This CTA's r-th item. The list's items shrink slowly (a prompt's tiles come last tile first), so the CTAs take them
-// in alternating order: 0..n-1, then n-1..0.
-SNB_DEVICE bool next_item(const PromptParams& p, int r, Item& it) {
+// This CTA's r-th item. The list's items mostly shrink slowly (a prompt's tiles come last tile first), so the CTAs take
+// them in alternating order: 0..n-1, then n-1..0.
+SNB_DEVICE bool next_item(const PromptParams& p, int r, Cursor& at, Item& it) {
   const int n = gridDim.x;
   const int64_t w = (int64_t)r * n + ((r & 1) ? n - 1 - blockIdx.x : blockIdx.x);
-  return w < p.items && decode_item(p, (int)w, it);
+  return w < p.items && decode_item(p, (int)w, at, it);
 }
 
 template <typename T, int D, int DV>
@@ -414,9 +420,10 @@ __global__ void __launch_bounds__(THREADS, 1)
   if (warp == LOAD_WARP) {
     int nq = 0, nk = 0, nv = 0;
     bool ok = true;
+    Cursor cursor;
     // It alone works the items out (a few global reads and divisions) and hands them over one item ahead.
     auto publish = [&](int r, Item& it) {
-      const bool have = next_item(p, r, it);
+      const bool have = next_item(p, r, cursor, it);
       if (!have) it.kb0 = it.kb1 = 0;
       if (lane == 0) {
         float sink[2] = {0.f, 0.f};
@@ -633,7 +640,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         auto next_chunk = [&](auto cut, int c, bool more) {
           snb::tmem_ld_wait();
           if (more) tmem_ld_x16(s_at + ((c + 1) & 3) * 16, s[(c + 1) & 1]);
-          if (cut.value && sight(c) < 2) {
+          if (cut.value && sight(c) == 1) {  // of those that no row sees the caller makes nothing
             const uint32_t seen = upto(rel - k0 - c * 16) & ~upto(lo - 1 - k0 - c * 16);
 #pragma unroll
             for (int i = 0; i < 16; ++i)
@@ -667,6 +674,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
               next_chunk(cut, c, true);
+              if (cut.value && sight(c) == 0) continue;
 #pragma unroll
               for (int i = 0; i < 16; i += 2)
                 mx[i / 2 & 1] = max3(mx[i / 2 & 1], __uint_as_float(s[c & 1][i]), __uint_as_float(s[c & 1][i + 1]));
