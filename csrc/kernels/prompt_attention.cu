@@ -11,8 +11,8 @@
 // What bounds it: the softmax warps. A block of both tiles is 2048 cycles of tensor core at head width 128 and takes
 // about 2600; per score they spend 0.75 exponentials of the special-function unit's 1/4 a cycle and scheduler (the rest
 // runs on the FMA pipe), the packing to 16 bits and the sums. Measured on a B200 (device time): one 8192-token prompt,
-// 32 / 8 heads of 128: 424 us, 1297 TFLOP/s; 64 / 8 heads of 64: 642 us, 857 TFLOP/s (the same scores at half the
-// products); 16 heads of 192 / 128: 332 us, 1035 TFLOP/s.
+// 32 / 8 heads of 128: 427 us, 1287 TFLOP/s; 64 / 8 heads of 64: 646 us, 850 TFLOP/s (the same scores at half the
+// products); 16 heads of 192 / 128: 333 us, 1031 TFLOP/s; 4096 tokens, 64 / 8 heads of 64, window 128: 44 us.
 // Tried and slower: one thread per row (its chain of loads, maximum, exponentials is twice as long: 575 us); turns of
 // the two tiles at the exponentials (with one thread per row 4 % faster, with two a loss); heads of 64 with one tile
 // per CTA and two CTAs per SM (687 us against 650).
