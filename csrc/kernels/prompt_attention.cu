@@ -647,7 +647,8 @@ __global__ void __launch_bounds__(THREADS, 1)
               if (!(seen >> i & 1)) s[c & 1][i] = 0xff800000u;
           }
         };
-        // The output in tensor memory follows a change of the reference by 2^-d, after the product `phase`.
+        // The output in tensor memory follows a change of the reference by 2^-d, after the product `phase`. The stores
+        // have landed on return: after an item's last block the epilogue reads the same columns with nothing in between.
         auto rescale = [&](float f, int phase) {
           ok = wait(&o_full[j], phase & 1);
 #pragma unroll 1
@@ -659,6 +660,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
             tmem_st_x32(o_at + c * 32, o);
           }
+          tmem_st_wait();
         };
         // Blocks that every row sees whole take a path without the tests: those cost as much as the exponentials.
         const bool ragged = kb * BKV + BKV - 1 > r0 || (p.window > 0 && kb * BKV < r0 + BQ - p.window);

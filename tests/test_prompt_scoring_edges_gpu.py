@@ -1,0 +1,50 @@
+"""Edge cases of the prompt-scoring kernels against plain implementations in 64 bits; the tolerances are those that
+test_prompt_scoring_gpu.py derives."""
+import math
+
+import pytest
+import torch
+
+from test_prompt_scoring_gpu import U, _attend64, _check_attention, _indptr, _qkv
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- attention ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("layout", [(2, 1, 128, 128), (3, 1, 64, 64), (2, 2, 192, 128)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("jump", [12.0, 40.0, 90.0])
+def test_prompt_attention_scores_jump_in_the_last_block(layout, dtype, jump):
+    """The scores rise by 2^jump in weight in the last block of keys only: the output is rescaled right before it is
+    read."""
+    from sglang_neuron_b200.ops.prompt import prompt_attention
+    Hq, Hkv, D, Dv = layout
+    lens = [129, 256, 200, 300, 384, 100]
+    q, k, v = (x.clone() for x in _qkv(sum(lens), Hq, Hkv, D, Dv, dtype, seed=int(jump)))
+    q[:] = 1.0
+    # scores in units of log 2: 0 before the last block, `jump` in it, a few units of noise
+    k.mul_(0.25)
+    at = 0
+    for n in lens:
+        last = at + (n - 1) // 128 * 128
+        k[last:at + n] += jump * math.log(2.0) / math.sqrt(D)
+        at += n
+    out = prompt_attention(q, k, v, _indptr(lens), Hq, Hkv, D, v_head_dim=Dv)
+    _check_attention(out, q, k, v, lens, Hq, Hkv, D, Dv)
+
+
+def test_prompt_attention_scores_jump_beside_rows_without_a_score():
+    """Rows of one warp whose first block holds only scores of -inf beside rows that are rescaled."""
+    from sglang_neuron_b200.ops.prompt import prompt_attention
+    n, Hq, Hkv, D = 384, 2, 1, 64
+    q, k, v = (x.clone() for x in _qkv(n, Hq, Hkv, D, D, torch.bfloat16, seed=31))
+    q[::2] = 1.0  # the first block's scores leave fp32's range
+    q[1::2] = 2.0 ** -126  # -16 there, 0 elsewhere
+    k[:128] = -(2.0 ** 127)
+    k[128:] = k[128:] * 0.25
+    k[256:] += 20 * math.log(2.0) / math.sqrt(D)
+    out = prompt_attention(q, k, v, _indptr([n]), Hq, Hkv, D)
+    want, A = _attend64(q, k, v, [n], Hq, Hkv, D, D, 0, D ** -0.5, None)
+    tol = (2 * U[q.dtype] + 4e-4) * A + n * 2.0 ** -24 * v.float().abs().max().item()
+    # in 64 bits the first block's scores stay finite: rows that see later keys compare
+    assert ((out.double() - want).abs() <= tol)[128:].all()
