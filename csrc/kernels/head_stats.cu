@@ -217,6 +217,7 @@ __global__ void __launch_bounds__(THREADS)
       float c = -INFINITY, s = 0.f, t = 0.f, chosen = -INFINITY;
 #pragma unroll 1
       for (int j = 0; j < p.width / 32; ++j) {
+        __syncwarp();  // the rows part below; the tensor-memory load wants the whole warp
         uint32_t r[32];
         snb::tmem_ld_32x32b_x32(tmem + ((uint32_t)(q * 32) << 16) + (n & 1) * BN + j * 32, r);
         snb::tmem_ld_wait();
@@ -234,19 +235,20 @@ __global__ void __launch_bounds__(THREADS)
           for (int i = 0; i < 32; ++i)
             if (id == j * 32 + i) chosen = __uint_as_float(r[i]);
         }
-        if (mx == -INFINITY) continue;
-        if (!(mx <= c)) {
-          const float f = ex2((c - mx) * LOG2E);
-          t = f > 0.f ? f * (t + s * (c - mx)) : 0.f;
-          s *= f;
-          c = mx;
-        }
+        if (mx != -INFINITY) {
+          if (!(mx <= c)) {
+            const float f = ex2((c - mx) * LOG2E);
+            t = f > 0.f ? f * (t + s * (c - mx)) : 0.f;
+            s *= f;
+            c = mx;
+          }
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const float y = max_nan(__uint_as_float(r[i]) - c, -1e30f);
-          const float e = ex2(y * LOG2E);
-          s += e;
-          t = fmaf(e, y, t);
+          for (int i = 0; i < 32; ++i) {
+            const float y = max_nan(__uint_as_float(r[i]) - c, -1e30f);
+            const float e = ex2(y * LOG2E);
+            s += e;
+            t = fmaf(e, y, t);
+          }
         }
       }
       snb::tc_fence_before();
@@ -418,6 +420,7 @@ __global__ void __launch_bounds__(THREADS)
       const int v = (g + q) * GROUP + lane;  // this lane's vocabulary entry
 #pragma unroll 1
       for (int j = 0; j < p.cols; j += 32) {
+        __syncwarp();
         uint32_t r[32];
         snb::tmem_ld_32x32b_x32(tmem + ((uint32_t)(q * 32) << 16) + (n & 1) * FEW + j, r);
         snb::tmem_ld_wait();

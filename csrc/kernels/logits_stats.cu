@@ -228,6 +228,7 @@ __global__ void __launch_bounds__(THREADS, 4)
     snb::fence_mbar_init();
   }
   // the first CTA's memory is written from the others: all of them have to be there by then
+  __syncwarp();
   if (C > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   __syncthreads();
   snb::pdl_wait();

@@ -643,8 +643,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           if (cut.value && sight(c) == 1) {  // of those that no row sees the caller makes nothing
             const uint32_t seen = upto(rel - k0 - c * 16) & ~upto(lo - 1 - k0 - c * 16);
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-              if (!(seen >> i & 1)) s[c & 1][i] = 0xff800000u;
+            for (int i = 0; i < 16; ++i) s[c & 1][i] = (seen >> i & 1) ? s[c & 1][i] : 0xff800000u;
           }
         };
         // The output in tensor memory follows a change of the reference by 2^-d, after the product `phase`. The stores
@@ -735,6 +734,7 @@ __global__ void __launch_bounds__(THREADS, 1)
               snb::tc_fence_before();
               __syncwarp();
               if (lane == 0) snb::mbar_arrive(&p_full[2 * j + c / 2]);
+              __syncwarp();  // the tensor-memory instructions want the whole warp
             }
           }
         };
@@ -797,6 +797,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                   make_uint4(w2[4 * i], w2[4 * i + 1], w2[4 * i + 2], w2[4 * i + 3]);
           }
         }
+        __syncwarp();
       }
       const bool odd = zero != 0.f;
       // A NaN or infinity in a masked value still meets a weight of 0 in the product (0 * inf = NaN), and a masked

@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from test_prompt_scoring_gpu import U, _attend64, _check_attention, _indptr, _qkv
+from test_prompt_scoring_gpu import (DEV, U, _attend64, _check_attention, _head, _indptr, _near, _qkv, _stats64)
 
 pytestmark = pytest.mark.gpu
 
@@ -48,3 +48,25 @@ def test_prompt_attention_scores_jump_beside_rows_without_a_score():
     tol = (2 * U[q.dtype] + 4e-4) * A + n * 2.0 ** -24 * v.float().abs().max().item()
     # in 64 bits the first block's scores stay finite: rows that see later keys compare
     assert ((out.double() - want).abs() <= tol)[128:].all()
+
+
+# ---- log-probabilities from hidden rows ---------------------------------------------------------------------
+@pytest.mark.parametrize("N", [70, 300])
+def test_head_logprobs_logits_of_minus_infinity_in_some_rows(N):
+    """Columns whose logits are -inf for some rows of a warp and ordinary for the others."""
+    from sglang_neuron_b200.ops.logprobs import head_logprobs
+    H, V = 128, 1000
+    h, w, ids = _head(N, H, V, torch.bfloat16, seed=N)
+    low = torch.zeros(N, dtype=torch.bool, device=DEV)
+    low[3::5] = True
+    dark = torch.zeros(V, dtype=torch.bool, device=DEV)
+    dark[32:64] = dark[100:420] = dark[999:] = True
+    h[:, 0] = w[:, 0] = 0
+    z = h.double() @ w.double().t()
+    tol = 3e-4 + (H / 16 + 4) * 2.0 ** -23 * (h.double().abs() @ w.double().abs().t()).max().item()
+    z[low[:, None] & dark[None, :]] = -math.inf
+    h[low, 0], w[dark, 0] = -3e38, 3e38  # their product leaves fp32's range
+    r = head_logprobs(h, w, ids)
+    lp, ent, lse, _, _ = _stats64(z, ids, 0)
+    assert _near(r.logprobs, lp, 2 * tol) and _near(r.lse, lse, tol)
+    assert _near(r.entropy, ent, 3e-4 + 3e-6 * 128 + 8 * tol)
