@@ -101,14 +101,16 @@ SNB_DEVICE float min_nan(float a, float b) {
 }
 
 // 2^x of two values on the FMA pipe: x = n + f with n the nearest integer (found by adding 1.5 * 2^23) and |f| <= 1/2,
-// 2^f by the cubic whose largest relative error on that interval is least (7.5e-5, by Remez exchange; weights are
-// rounded to 2^-9 or 2^-12 next), n added to the exponent. Below -125 the result is 2^-125; 128 and above (`HIGH`: x
-// can get there) and NaN become values past every 16-bit type's range.
+// 2^f by the cubic with p(0) = 1 whose largest relative error on that interval is least (1.02e-4, by Remez exchange;
+// weights are rounded to 2^-9 or 2^-12 next), n added to the exponent. At -127 and below, masked scores of -inf among
+// them, the result is exactly 0 (p(0) = 1 has no mantissa, and the exponent is 0), so what is masked adds nothing; down
+// to -126 it is a value below 2^-126. 128 and above (`HIGH`: x can get there) and NaN become values past every 16-bit
+// type's range.
 template <bool HIGH>
 SNB_DEVICE float2 exp2_fma(uint64_t x) {
   float2 c = split(x);
-  c.x = max_nan(c.x, -125.f);
-  c.y = max_nan(c.y, -125.f);
+  c.x = max_nan(c.x, -127.f);
+  c.y = max_nan(c.y, -127.f);
   if (HIGH) {
     c.x = min_nan(c.x, 128.f);
     c.y = min_nan(c.y, 128.f);
@@ -117,9 +119,9 @@ SNB_DEVICE float2 exp2_fma(uint64_t x) {
   const uint64_t big = pair(12582912.f, 12582912.f), less = pair(-12582912.f, -12582912.f);
   const uint64_t n = add2(x, big);
   const uint64_t f = fma2(add2(n, less), pair(-1.f, -1.f), x);
-  uint64_t y = fma2(pair(0.05517166852953102f, 0.05517166852953102f), f, pair(0.2426111251115799f, 0.2426111251115799f));
-  y = fma2(y, f, pair(0.6932609677314758f, 0.6932609677314758f));
-  y = fma2(y, f, pair(0.9999280571937561f, 0.9999280571937561f));
+  uint64_t y = fma2(pair(0.055009059607982635f, 0.055009059607982635f), f, pair(0.2422109693288803f, 0.2422109693288803f));
+  y = fma2(y, f, pair(0.6932829022407532f, 0.6932829022407532f));
+  y = fma2(y, f, pair(1.f, 1.f));
   const float2 ny = split(n), r = split(y);
   return make_float2(__int_as_float(__float_as_int(r.x) + (__float_as_int(ny.x) << 23)),
                      __int_as_float(__float_as_int(r.y) + (__float_as_int(ny.y) << 23)));

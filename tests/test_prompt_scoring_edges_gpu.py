@@ -50,6 +50,52 @@ def test_prompt_attention_scores_jump_beside_rows_without_a_score():
     assert ((out.double() - want).abs() <= tol)[128:].all()
 
 
+@pytest.mark.parametrize("layout", [(4, 2, 64, 64), (3, 1, 128, 128), (2, 2, 192, 128)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("window", [0, 50])
+@pytest.mark.parametrize("huge", [1e4, 1e30, 3e38])
+def test_prompt_attention_masked_values_weigh_nothing(layout, dtype, window, huge):
+    """Huge finite values, which no recomputing of infinite results catches: rows that do not see them keep their
+    bits, and so do rows beside tokens of no prompt."""
+    from sglang_neuron_b200.ops.prompt import prompt_attention
+    if dtype == torch.float16:
+        huge = min(huge, 6e4)
+    Hq, Hkv, D, Dv = layout
+    lens = [100, 190, 150]
+    T = sum(lens) + 40  # the last 40 tokens belong to no prompt
+    q, k, v = (x.clone() for x in _qkv(T, Hq, Hkv, D, Dv, dtype, seed=9))
+    ip = _indptr(lens)
+    clean = prompt_attention(q, k, v, ip, Hq, Hkv, D, v_head_dim=Dv, window=window)[:sum(lens)]
+    hit = torch.zeros(sum(lens), dtype=torch.bool, device=DEV)
+    for t, end in ((30, 100), (100 + 77, 290), (290 + 149, 440)):
+        v[t] = huge
+        hit[t:min(end, t + window) if window else end] = True
+    v[sum(lens):] = -huge
+    out = prompt_attention(q, k, v, ip, Hq, Hkv, D, v_head_dim=Dv, window=window)[:sum(lens)]
+    assert torch.equal(out[~hit], clean[~hit])
+
+
+def test_prompt_attention_seen_scores_of_minus_infinity_weigh_nothing():
+    """A key that scores -inf has weight 0 also where the row sees it, whatever finite value it holds."""
+    from sglang_neuron_b200.ops.prompt import prompt_attention
+    n, Hq, Hkv, D = 300, 2, 1, 64
+    q, k, v = (x.clone() for x in _qkv(n, Hq, Hkv, D, D, torch.bfloat16, seed=12))
+    q = q.abs() + 0.1
+    clean_k, clean_v = k.clone(), v.clone()
+    k[2::5], v[2::5] = -math.inf, 3e38
+    keep = torch.ones(n, dtype=torch.bool, device=DEV)
+    keep[2::5] = False
+    out = prompt_attention(q, k, v, _indptr([n]), Hq, Hkv, D)
+    # in 64 bits: the prompt without those keys, a row of it at every kept token
+    s = torch.einsum("qhd,kd->hqk", q.double().view(n, Hq, D), clean_k.double()) * D ** -0.5
+    t = torch.arange(n, device=DEV)
+    s.masked_fill_((t[None, :] > t[:, None]) | ~keep[None, :], -math.inf)
+    p = torch.softmax(s, -1)
+    want = torch.einsum("hqk,kd->qhd", p, clean_v.double()).reshape(n, -1)
+    A = torch.einsum("hqk,kd->qhd", p, clean_v.double().abs()).reshape(n, -1)
+    assert ((out.double() - want).abs() <= (2 * U[q.dtype] + 4e-4) * A + 1e-6).all()
+
+
 # ---- log-probabilities from hidden rows ---------------------------------------------------------------------
 @pytest.mark.parametrize("N", [70, 300])
 def test_head_logprobs_logits_of_minus_infinity_in_some_rows(N):
