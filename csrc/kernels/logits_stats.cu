@@ -15,9 +15,11 @@
 //
 // Bound: the logits' bytes at DRAM rate. A bf16 row at that rate brings 12 logits a clock and SM, so a logit has one
 // exponential (of 16 a clock) and few issue slots: two values go through each fp32 instruction (f32x2), y is taken in
-// units of log 2 by one multiply-add, maximum and floor act on the 16-bit pairs as loaded. The floor (-2^100, fp16
-// -6e4) keeps 0 * y finite where a logit is masked; a CTA whose every logit lies down there reads its part once more
-// on an exact path.
+// units of log 2 by one multiply-add, maximum and floor act on the 16-bit pairs as loaded. The reference is rounded
+// before it is subtracted, which shifts y by up to 2^-25 of the reference; the end takes that out again, and up to 2^26
+// the shift is at most 4. So logits count as at least -2^26 (fp16 -6e4), which weighs nothing beside a maximum above
+// -2^25 and keeps 0 * y finite where a logit is masked; a CTA whose maximum is outside +-2^25 (LOWEST, HIGHEST) reads
+// its part once more on a path that subtracts first.
 // The row comes through a ring of three 16 KB bulk copies that one thread keeps full.
 // Measured on a B200: 4096 x 151936 bf16 without alternatives 234 us (5.3 TB/s), with five 254 us, with twenty 301 us
 // (choosing them takes a CTA some 5 us after its row); 1000 x 201088 fp32 with five 135 us (6.0 TB/s); 64 x 201088 fp32
@@ -108,7 +110,7 @@ struct Vec;
 template <>
 struct Vec<float> {
   static constexpr int N = 4;
-  static constexpr float FLOOR = -0x1p100f, LOWEST = -0x1p99f;
+  static constexpr float FLOOR = -0x1p26f, LOWEST = -0x1p25f, HIGHEST = 0x1p25f;
   static constexpr uint32_t NONE = 0xff800000u;
   static SNB_DEVICE float2 two(const uint4& u, int i) {
     return i == 0 ? make_float2(__uint_as_float(u.x), __uint_as_float(u.y))
@@ -143,7 +145,7 @@ struct Vec16 {
 };
 template <>
 struct Vec<__nv_bfloat16> : Vec16<__nv_bfloat16, __nv_bfloat162> {
-  static constexpr float FLOOR = -0x1p100f, LOWEST = -0x1p99f;
+  static constexpr float FLOOR = -0x1p26f, LOWEST = -0x1p25f, HIGHEST = 0x1p25f;
   static constexpr uint32_t NONE = 0xff80ff80u;
   static SNB_DEVICE float2 two(const uint4& u, int i) {
     const uint32_t w = word(u, i);
@@ -158,7 +160,7 @@ struct Vec<__nv_bfloat16> : Vec16<__nv_bfloat16, __nv_bfloat162> {
 };
 template <>
 struct Vec<__half> : Vec16<__half, __half2> {
-  static constexpr float FLOOR = -6e4f, LOWEST = -5.9e4f;
+  static constexpr float FLOOR = -6e4f, LOWEST = -5.9e4f, HIGHEST = 0x1p16f;
   static constexpr uint32_t NONE = 0xfc00fc00u;
   static SNB_DEVICE float2 two(const uint4& u, int i) { return __half22float2(as(word(u, i))); }
   static SNB_DEVICE float maximum(const uint4& u) {
@@ -348,7 +350,7 @@ __global__ void __launch_bounds__(THREADS, 4)
     st_s += e;
     st_t = fmaf(e, y, st_t);
   };
-  if (most <= Vec<T>::LOWEST || most > 1e30f) {
+  if (most <= Vec<T>::LOWEST || most > Vec<T>::HIGHEST) {
     if (warp < WARPS && most != -INFINITY)
       for (int u = u0 + warp; u < u1; u += WARPS) {
         if (u * 32 + lane >= cut.nvec) continue;

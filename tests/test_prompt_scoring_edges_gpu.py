@@ -5,7 +5,8 @@ import math
 import pytest
 import torch
 
-from test_prompt_scoring_gpu import (DEV, U, _attend64, _check_attention, _head, _indptr, _near, _qkv, _stats64)
+from test_prompt_scoring_gpu import (DEV, U, _attend64, _check_attention, _check_stats, _head, _indptr, _near,
+                                     _qkv, _stats64)
 
 pytestmark = pytest.mark.gpu
 
@@ -94,6 +95,34 @@ def test_prompt_attention_seen_scores_of_minus_infinity_weigh_nothing():
     want = torch.einsum("hqk,kd->qhd", p, clean_v.double()).reshape(n, -1)
     A = torch.einsum("hqk,kd->qhd", p, clean_v.double().abs()).reshape(n, -1)
     assert ((out.double() - want).abs() <= (2 * U[q.dtype] + 4e-4) * A + 1e-6).all()
+
+
+# ---- log-probabilities from logits --------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("N", [1, 700])
+@pytest.mark.parametrize("big", [1e6, 3e7, 1e9, 1e10, 1e15, 1e20, 1e30, 1e34])
+def test_token_logprobs_large_finite_logits(dtype, N, big):
+    """Masks of finite values between the ordinary and the type's lowest, and rows at such a level."""
+    from sglang_neuron_b200.ops.logprobs import token_logprobs
+    V = 30011
+    g = torch.Generator(device=DEV).manual_seed(N)
+    x = (torch.randn(N, V, device=DEV, generator=g) * 3).to(dtype)
+    ids = torch.randint(0, V, (N,), device=DEV, generator=g)
+    # long masked stretches before, between and after the ordinary logits; a lone ordinary logit at the end
+    y = x.clone()
+    y[:, :20000] = -big
+    y[:, 20100:29000] = -big
+    z = torch.full_like(x, -big)
+    z[:, -1] = 1.5
+    up = x.clone()
+    up[:, 5000:5003] = big  # far above the rest
+    for t, i in ((y, ids.clamp(29000, V - 1)), (y, ids), (z, ids), (up, torch.full_like(ids, 5001)), (up, ids)):
+        _check_stats(token_logprobs(t, i, top_k=5), t, i, 5)
+    for c in (big, -big):
+        t = torch.full_like(x, c)
+        _check_stats(token_logprobs(t, ids, top_k=32), t, ids, 32)
+        t[:, 77] = c * 1.25
+        _check_stats(token_logprobs(t, ids, top_k=3), t, ids, 3)
 
 
 # ---- log-probabilities from hidden rows ---------------------------------------------------------------------
