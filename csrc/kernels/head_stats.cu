@@ -582,7 +582,6 @@ int pick_width(int mt, int64_t V, int pairs) {
 std::tuple<at::Tensor, at::Tensor, at::Tensor> head_stats(at::Tensor hidden, at::Tensor weight, int64_t F, bool tiled,
                                                           int64_t V, at::Tensor ids, int64_t vocab_offset,
                                                           at::Tensor status) {
-  // plain messages: putting numbers into them needs streams that this extension does not bring along
   TORCH_CHECK(hidden.is_cuda() && hidden.dim() == 2 && weight.dim() == 2 &&
                   (tiled || hidden.size(1) == weight.size(1)),
               "head_logprobs: hidden [rows, size] does not fit the weight [vocabulary, size]");

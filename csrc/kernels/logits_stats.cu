@@ -608,7 +608,6 @@ void launch(const at::Tensor& logits, int V, const at::Tensor& ids, int64_t voca
 // log-probability, entropy and log-sum-exp, the K best log-probabilities [N, K] and their ids.
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> logits_stats(
     at::Tensor logits, int64_t V, at::Tensor ids, int64_t vocab_offset, int64_t K, at::Tensor status) {
-  // plain messages: putting numbers into them needs streams that this extension does not bring along
   TORCH_CHECK(logits.is_cuda() && logits.dim() == 2, "token_logprobs: logits must be [rows, vocabulary] on CUDA");
   const int64_t N = logits.size(0);
   if (V == 0) V = logits.size(1);

@@ -879,7 +879,6 @@ bool is_matrix(const at::Tensor& x, int64_t T, int64_t width, const at::Tensor& 
 at::Tensor prompt_attention(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor indptr, int64_t heads,
                             int64_t kv_heads, int64_t D, int64_t DV, int64_t window, double sm_scale,
                             std::optional<at::Tensor> sinks, std::optional<at::Tensor> given, at::Tensor status) {
-  // the messages are plain text: putting numbers into them needs streams that this extension does not bring along
   TORCH_CHECK(q.is_cuda() && q.dim() == 2, "prompt_attention: q must be a CUDA matrix");
   TORCH_CHECK(heads > 0 && kv_heads > 0 && heads % kv_heads == 0,
               "prompt_attention: the heads do not divide over the KV heads");

@@ -30,6 +30,11 @@ NVCC_FLAGS = ARCH + [
 if os.environ.get("SNB_PTXAS_VERBOSE"):
     NVCC_FLAGS.append("-Xptxas=-v")
 
+# The process has one C++ runtime, the shared one that torch loads. Named outright, because where the compiler finds only
+# the static archive, -lstdc++ puts a second runtime into each extension, and formatting a number through two of them
+# (a check's message) ended the process.
+LINK_FLAGS = ["-l:libstdc++.so.6"]
+
 kernel_sources = sorted(glob.glob(os.path.join("csrc", "kernels", "*.cu"))) + ["csrc/bindings.cpp"]
 runtime_sources = sorted(glob.glob(os.path.join("csrc", "runtime", "*.cpp")))
 
@@ -39,6 +44,7 @@ ext_modules = [
         sources=kernel_sources,
         include_dirs=[os.path.join(ROOT, "csrc")],
         extra_compile_args={"cxx": ["-O3", "-std=c++17"], "nvcc": NVCC_FLAGS},
+        extra_link_args=LINK_FLAGS,
     ),
 ]
 if runtime_sources:
@@ -48,6 +54,7 @@ if runtime_sources:
             sources=runtime_sources,
             include_dirs=[os.path.join(ROOT, "csrc")],
             extra_compile_args=["-O3", "-std=c++17"],
+            extra_link_args=LINK_FLAGS,
             libraries=["rt"],  # shm_open on older glibc
         )
     )
