@@ -599,14 +599,11 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> head_stats(at::Tensor hidden, at:
               "head_logprobs: ids must be one int64 or int32 per row on the rows' device");
   TORCH_CHECK(N < (int64_t(1) << 30), "head_logprobs: too many rows");
   const c10::cuda::CUDAGuard guard(hidden.device());
-  auto readable = [](const at::Tensor& x) {
-    return x.stride(1) == 1 && x.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
-  };
   auto stats = at::empty({3, N}, hidden.options().dtype(at::kFloat));
   const auto result = std::make_tuple(stats.select(0, 0), stats.select(0, 1), stats.select(0, 2));
   if (N == 0) return result;
-  if (!readable(hidden)) hidden = hidden.contiguous();
-  if (!readable(weight)) weight = weight.contiguous();
+  hidden = snb_host::mappable(hidden);
+  weight = snb_host::mappable(weight);
   ids = ids.to(at::kLong).contiguous();
   const bool bf16 = hidden.scalar_type() == at::kBFloat16;
   const auto dt = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;

@@ -862,10 +862,6 @@ void dispatch(const PromptParams& p, int64_t D, int64_t DV, int* status, cudaStr
   else TORCH_CHECK(false, "prompt_attention: serves keys / values 64 / 64, 128 / 128 or 192 / 128 wide");
 }
 
-bool readable(const at::Tensor& x) {  // contiguous rows on 16-byte boundaries
-  return x.stride(1) == 1 && x.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
-}
-
 bool is_matrix(const at::Tensor& x, int64_t T, int64_t width, const at::Tensor& q) {
   return x.dim() == 2 && x.size(0) == T && x.size(1) == width && x.scalar_type() == q.scalar_type() &&
          x.device() == q.device();
@@ -873,9 +869,9 @@ bool is_matrix(const at::Tensor& x, int64_t T, int64_t width, const at::Tensor& 
 
 }  // namespace
 
-// q [T, heads * D], k [T, kv_heads * D], v [T, kv_heads * DV]: bf16 or fp16 (rows that are not contiguous or not on
-// 16-byte boundaries are copied first); out [T, heads * DV] or none. indptr [B + 1] int32, ascending; rows outside
-// every prompt are not written.
+// q [T, heads * D], k [T, kv_heads * D], v [T, kv_heads * DV]: bf16 or fp16 (rows that are not contiguous, not on
+// 16-byte boundaries or overlap are copied first); out [T, heads * DV] or none. indptr [B + 1] int32, ascending; rows
+// outside every prompt are not written.
 at::Tensor prompt_attention(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor indptr, int64_t heads,
                             int64_t kv_heads, int64_t D, int64_t DV, int64_t window, double sm_scale,
                             std::optional<at::Tensor> sinks, std::optional<at::Tensor> given, at::Tensor status) {
@@ -903,11 +899,13 @@ at::Tensor prompt_attention(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor
   at::Tensor out = given ? *given : at::empty({T, heads * DV}, q.options());
   TORCH_CHECK(is_matrix(out, T, heads * DV, q),
               "prompt_attention: out must be [tokens, heads * v_head_dim] of q's type and device");
-  TORCH_CHECK(T == 0 || readable(out), "prompt_attention: out needs contiguous rows on 16-byte boundaries");
+  // a single row's stride means nothing
+  TORCH_CHECK(T == 0 || snb_host::is_mappable(T > 1 ? out : out.view({heads * DV}).unsqueeze(0)),
+              "prompt_attention: out needs contiguous rows on 16-byte boundaries that do not overlap");
   if (T == 0 || B == 0) return out;
-  if (!readable(q)) q = q.contiguous();
-  if (!readable(k)) k = k.contiguous();
-  if (!readable(v)) v = v.contiguous();
+  q = snb_host::mappable(q);
+  k = snb_host::mappable(k);
+  v = snb_host::mappable(v);
   indptr = indptr.contiguous();
   PromptParams p;
   p.q = q.data_ptr();
@@ -917,7 +915,7 @@ at::Tensor prompt_attention(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor
   p.qs = q.stride(0);
   p.ks = k.stride(0);
   p.vs = v.stride(0);
-  p.os = out.stride(0);
+  p.os = T > 1 ? out.stride(0) : heads * DV;
   p.indptr = indptr.data_ptr<int>();
   p.sinks = sinks ? sinks->data_ptr<float>() : nullptr;
   p.T = (int)T;

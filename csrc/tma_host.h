@@ -4,6 +4,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <cudaTypedefs.h>
+#include <ATen/core/Tensor.h>
 #include <c10/util/Exception.h>
 
 namespace snb_host {
@@ -19,6 +20,17 @@ inline PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
     fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
   }
   return fn;
+}
+
+// Whether a matrix of 16-bit elements can be mapped as it is: contiguous rows on 16-byte boundaries that do not overlap.
+inline bool is_mappable(const at::Tensor& x) {
+  return x.stride(1) == 1 && x.stride(0) % 8 == 0 && x.stride(0) >= x.size(1) &&
+         reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
+}
+// The matrix, or a copy that can be mapped. A clone, since contiguous() keeps what counts as contiguous already: a
+// tensor off the boundaries, or a single row whatever its stride says.
+inline at::Tensor mappable(const at::Tensor& x) {
+  return is_mappable(x) ? x : x.clone(at::MemoryFormat::Contiguous);
 }
 
 // 2D tiled map over a row-major matrix: `inner` elements per row (contiguous), `outer` rows,

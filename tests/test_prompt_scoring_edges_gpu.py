@@ -97,6 +97,51 @@ def test_prompt_attention_seen_scores_of_minus_infinity_weigh_nothing():
     assert ((out.double() - want).abs() <= (2 * U[q.dtype] + 4e-4) * A + 1e-6).all()
 
 
+def _odd_views(x):
+    """The values of x in forms that tensor maps do not take as they are."""
+    n, w = x.shape
+    flat = torch.empty(n * w + 1, device=DEV, dtype=x.dtype)
+    flat[1:] = x.reshape(-1)
+    yield "contiguous, off the 16-byte boundaries", flat[1:].view(n, w)
+    wide = torch.empty(n, w + 3, device=DEV, dtype=x.dtype)
+    wide[:, :w] = x
+    yield "a row stride of its own", wide[:, :w]
+    yield "columns first", x.t().contiguous().t()
+
+
+@pytest.mark.parametrize("T", [1, 37])
+def test_prompt_attention_takes_any_rows(T):
+    from sglang_neuron_b200.ops.prompt import prompt_attention
+    Hq, Hkv, D = 4, 2, 64
+    qkv = [x.contiguous() for x in _qkv(T, Hq, Hkv, D, D, torch.bfloat16)]
+    ip = _indptr([T])
+    want = prompt_attention(*qkv, ip, Hq, Hkv, D)
+    for i in range(3):
+        for what, view in _odd_views(qkv[i]):
+            args = qkv[:i] + [view] + qkv[i + 1:]
+            assert torch.equal(prompt_attention(*args, ip, Hq, Hkv, D), want), (i, what)
+    # one row for all tokens
+    k1, v1 = (x[:1].expand(T, -1) for x in qkv[1:])
+    want = prompt_attention(qkv[0], k1.contiguous(), v1.contiguous(), ip, Hq, Hkv, D)
+    assert torch.equal(prompt_attention(qkv[0], k1, v1, ip, Hq, Hkv, D), want)
+
+
+def test_prompt_attention_output_rows():
+    from sglang_neuron_b200.ops.prompt import prompt_attention
+    Hq, Hkv, D = 4, 2, 64
+    q, k, v = (x.contiguous() for x in _qkv(3, Hq, Hkv, D, D, torch.bfloat16))
+    ip1, ip3 = _indptr([1]), _indptr([3])
+    want = prompt_attention(q[:1], k[:1], v[:1], ip1, Hq, Hkv, D)
+    # a single row's stride means nothing
+    one = torch.zeros(1, Hq * D + 3, device=DEV, dtype=q.dtype)[:, :Hq * D]
+    assert torch.equal(prompt_attention(q[:1], k[:1], v[:1], ip1, Hq, Hkv, D, out=one), want)
+    flat = torch.zeros(3 * Hq * D + 1, device=DEV, dtype=q.dtype)
+    for bad in (flat[1:].view(3, -1), flat[:Hq * D].expand(3, -1),
+                torch.zeros(3, Hq * D + 3, device=DEV, dtype=q.dtype)[:, :Hq * D]):
+        with pytest.raises(ValueError):
+            prompt_attention(q, k, v, ip3, Hq, Hkv, D, out=bad)
+
+
 # ---- log-probabilities from logits --------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("N", [1, 700])
@@ -145,3 +190,17 @@ def test_head_logprobs_logits_of_minus_infinity_in_some_rows(N):
     lp, ent, lse, _, _ = _stats64(z, ids, 0)
     assert _near(r.logprobs, lp, 2 * tol) and _near(r.lse, lse, tol)
     assert _near(r.entropy, ent, 3e-4 + 3e-6 * 128 + 8 * tol)
+
+
+@pytest.mark.parametrize("N", [1, 50, 200])
+@pytest.mark.parametrize("V", [1, 300])
+def test_head_logprobs_takes_any_rows(N, V):
+    from sglang_neuron_b200.ops.logprobs import head_logprobs
+    h, w, ids = _head(N, 136, V, torch.bfloat16)
+    want = head_logprobs(h, w, ids)
+    cases = [(what, view, w) for what, view in _odd_views(h)] + [(what, h, view) for what, view in _odd_views(w)]
+    cases += [("one row", h[:1].expand(N, -1), w)]
+    for what, hh, ww in cases:
+        ref = head_logprobs(hh.contiguous().clone(), w, ids) if what == "one row" else want
+        for a, b in zip(head_logprobs(hh, ww, ids)[:3], ref[:3]):
+            assert torch.equal(a, b), what
