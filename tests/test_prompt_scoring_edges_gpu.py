@@ -5,8 +5,8 @@ import math
 import pytest
 import torch
 
-from test_prompt_scoring_gpu import (DEV, U, _attend64, _check_attention, _check_stats, _head, _indptr, _near,
-                                     _qkv, _stats64)
+from test_prompt_scoring_gpu import (DEV, U, _attend64, _check_attention, _check_head, _check_stats, _head, _indptr,
+                                     _near, _qkv, _stats64)
 
 pytestmark = pytest.mark.gpu
 
@@ -204,3 +204,41 @@ def test_head_logprobs_takes_any_rows(N, V):
         ref = head_logprobs(hh.contiguous().clone(), w, ids) if what == "one row" else want
         for a, b in zip(head_logprobs(hh, ww, ids)[:3], ref[:3]):
             assert torch.equal(a, b), what
+
+
+@pytest.mark.parametrize("N", [70, 129, 300, 1000])
+@pytest.mark.parametrize("V", [1003, 8000, 9000, 10003, 12000, 15000])
+def test_head_logprobs_forms_of_the_weight(N, V):
+    """Both kernels (up to 128 rows, and more) at several tile widths: a vocabulary below the weight's rows with NaN
+    behind it, tiles, strided rows, int32 ids, a shard's offset, a row of NaN."""
+    from sglang_neuron_b200.ops.gemm import TiledWeight
+    from sglang_neuron_b200.ops.logprobs import head_logprobs
+    H = 200  # not a multiple of the 64 that a step of the contraction takes
+    h, w, ids = _head(N, H, V + 97, torch.bfloat16, seed=V)
+    ids = ids % V
+    ids[0], ids[-1] = 0, V - 1
+    w[V:] = math.nan
+    want = head_logprobs(h, w[:V], ids)
+    _check_head(want, h, w[:V], ids)
+    wide_h = torch.zeros(N, H + 8, device=DEV, dtype=h.dtype)
+    wide_h[:, 8:] = h
+    wide_w = torch.zeros(V + 97, H + 24, device=DEV, dtype=w.dtype)
+    wide_w[:, 16:16 + H] = w
+    for hh, ww in ((h, w), (wide_h[:, 8:], w), (h, wide_w[:, 16:16 + H]), (h, TiledWeight(w)),
+                   (wide_h[:, 8:], TiledWeight(w)), (h, TiledWeight(w, keep_rowmajor=True))):
+        r = head_logprobs(hh, ww, ids.int(), valid_vocab=V)
+        for a, b in zip(r[:3], want[:3]):
+            assert torch.equal(a, b)
+    for weight in (w, TiledWeight(w)):
+        r = head_logprobs(h, weight, ids + 5000, vocab_offset=5000, valid_vocab=V)
+        assert all(torch.equal(a, b) for a, b in zip(r[:3], want[:3]))
+        for off in (5000 + V, -V):  # every id before or behind the shard
+            r = head_logprobs(h, weight, ids, vocab_offset=off, valid_vocab=V)
+            assert bool((r.logprobs == -math.inf).all()) and torch.equal(r.lse, want.lse)
+            assert torch.equal(r.entropy, want.entropy)
+        h2 = h.clone()
+        h2[N // 2] = math.nan
+        r = head_logprobs(h2, weight, ids, valid_vocab=V)
+        keep = torch.arange(N, device=DEV) != N // 2
+        for a, b in zip(r[:3], want[:3]):
+            assert torch.equal(a[keep], b[keep]) and bool(torch.isnan(a[~keep]).all())
