@@ -165,7 +165,8 @@ class Engine:
 
     def score(self, prompts: Sequence, top_logprobs_num: int = 0) -> List[Dict]:
         """How likely the model finds each prompt: the log-probability of every token given the ones before it, the
-        entropy of each of those distributions and, with top_logprobs_num, the best alternatives (temperature 1).
+        entropy of each of those distributions and, with top_logprobs_num, the best alternatives (temperature 1). All
+        come from logits in fp32, with and without alternatives.
 
         Prompts (token-id lists or strings) run whole, packed up to max_prefill_tokens tokens a forward, without
         touching the KV cache or the scheduler. Per prompt: `input_token_logprobs` [[log-probability, id], ...]

@@ -329,13 +329,15 @@ class ModelRunner:
         ])
 
     # ------------------------------------------------------------------------------------------
-    # rows whose logits exist at a time when alternatives are asked for (0.8 GB of bf16 logits at 201088 tokens)
-    SCORE_ROWS = 2048
+    # rows whose logits exist at a time when alternatives are asked for (0.8 GB in fp32 at 201088 tokens)
+    SCORE_ROWS = 1024
 
     def score_prompts(self, prompts: List[List[int]], top_k: int = 0):
         """One forward over whole prompts packed one after another, without the KV pool: TokenLogprobs of every
         prompt's tokens after its first, in order, on the device. With alternatives (top_k > 0) the logits exist
-        for SCORE_ROWS rows at a time, without them not at all."""
+        for SCORE_ROWS rows at a time, without them not at all; in fp32 both times, so that the given tokens' scores do
+        not change with the alternatives."""
+        from ..ops.gemm import linear_fp32
         from ..ops.logprobs import TokenLogprobs, head_logprobs, token_logprobs
         lens = [len(p) for p in prompts]
         T = sum(lens)
@@ -362,8 +364,8 @@ class ModelRunner:
             local = head_logprobs(h, self.model.lm_head.gemm_weight, want, vocab_offset=off, valid_vocab=V)
         else:
             k = min(top_k, V)
-            parts = [token_logprobs(self.model.compute_logits(h[a:a + self.SCORE_ROWS]), want[a:a + self.SCORE_ROWS],
-                                    top_k=k, vocab_offset=off, valid_vocab=V)
+            parts = [token_logprobs(linear_fp32(h[a:a + self.SCORE_ROWS], self.model.lm_head.gemm_weight),
+                                    want[a:a + self.SCORE_ROWS], top_k=k, vocab_offset=off, valid_vocab=V)
                      for a in range(0, len(rows), self.SCORE_ROWS)]
             local = TokenLogprobs(*(torch.cat(t) for t in zip(*parts)))
             if k < top_k:  # a shard smaller than the alternatives asked for

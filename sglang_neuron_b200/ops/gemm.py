@@ -139,6 +139,17 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None
     return out.view(*shape[:-1], F)
 
 
+def linear_fp32(x: torch.Tensor, w) -> torch.Tensor:
+    """x @ w.T with the products' fp32 sums kept (fp64 stays fp64). x: [T, K], w: [F, K] tensor or TiledWeight."""
+    if isinstance(w, TiledWeight):
+        if w.rowmajor is None and x.is_cuda and w.K > 64:
+            return linear_partials(x.contiguous(), w, 2).view(2, x.shape[0], w.F).sum(0)
+        w = w.rowmajor if w.rowmajor is not None else w.untiled()
+    if x.dtype in (torch.float32, torch.float64):
+        return x @ w.t()
+    return torch.mm(x, w.t(), out_dtype=torch.float32) if x.is_cuda else x.float() @ w.float().t()
+
+
 def linear_partials(x2: torch.Tensor, w: torch.Tensor, splits: int) -> torch.Tensor:
     """Split-K fp32 partial products [splits, T, F] of x2 @ w.T, left unreduced (a fused reduce follows)."""
     wk, F, tiled_f = _weight_args(w)
