@@ -63,6 +63,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, qo_indpt
     r = prompt_attention_ref(q, k, v, qo_indptr, num_q_heads, num_kv_heads, head_dim, v_head_dim, window, sm_scale,
                              sinks).to(q.dtype)
     if out is not None:
-        out.copy_(r)
+        for a, b in zip(qo_indptr[:-1].tolist(), qo_indptr[1:].tolist()):
+            out[a:b] = r[a:b]
         return out
     return r
