@@ -42,7 +42,15 @@ def _attend_ref(q, k, v, q_pos, k_pos, sm_scale, window, sinks):
     p = p / torch.where(denom > 0, denom, torch.ones_like(denom))
     if sinks is not None:
         p = p[..., :-1]
-    return torch.einsum("hqk,khd->qhd", p, v)
+    bad = ~torch.isfinite(v)
+    if not bool(bad.any()):
+        return torch.einsum("hqk,khd->qhd", p, v)
+    # a NaN or infinity reaches the rows that see it only (0 * NaN would reach them all)
+    out = torch.einsum("hqk,khd->qhd", p, v.masked_fill(bad, 0.0))
+    for j in bad.flatten(1).any(1).nonzero()[:, 0].tolist():
+        rows = allowed[:, j]
+        out[rows] += torch.where(bad[j], p[:, rows, j].t()[:, :, None] * v[j], torch.zeros_like(v[j]))
+    return out
 
 
 def decode_attention_ref(q, k_cache, v_cache, block_table, seq_lens, num_q_heads, num_kv_heads, head_dim,
