@@ -3,9 +3,9 @@
 logits).
 
 Both describe the distribution at temperature 1 over the first `valid_vocab` columns; what later (padding) columns
-hold does not matter. With a vocabulary-sharded head every rank calls them on its own shard with its first token id
-as `vocab_offset` and `merge_shards` joins the ranks' results. Parity: the reference sampler's per-shard logsumexp
-and exact top-logprobs (sglang_neuron/sampling.py:212-470).
+hold does not matter. Forward only: results carry no gradient, on CUDA or CPU. With a vocabulary-sharded head every
+rank calls them on its own shard with its first token id as `vocab_offset` and `merge_shards` joins the ranks' results.
+Parity: the reference sampler's per-shard logsumexp and exact top-logprobs (sglang_neuron/sampling.py:212-470).
 """
 from typing import NamedTuple
 
@@ -28,6 +28,7 @@ class TokenLogprobs(NamedTuple):
     top_ids: torch.Tensor        # [N, top_k] int64
 
 
+@torch.no_grad()
 def token_logprobs_ref(logits: torch.Tensor, ids: torch.Tensor, top_k: int = 0, vocab_offset: int = 0,
                        valid_vocab: int = 0) -> TokenLogprobs:
     V = valid_vocab or logits.shape[1]

@@ -1,7 +1,7 @@
 """Causal attention of packed whole prompts: keys and values straight from the projections, no paged cache.
 
-For passes that keep nothing (scoring prompts) and for the first pass of whole prompts. GQA, sliding window and
-learned per-head sinks as in the paged ops (ops/attention.py); the value width may differ from the key width
+For passes that keep nothing (scoring prompts). Forward only: results carry no gradient, on CUDA or CPU. GQA, sliding
+window and learned per-head sinks as in the paged ops (ops/attention.py); the value width may differ from the key width
 (decompressed latent attention: 192 / 128).
 """
 from typing import Optional
@@ -13,6 +13,7 @@ from .attention import _attend_ref
 from .gemm import _status_buf
 
 
+@torch.no_grad()
 def prompt_attention_ref(q, k, v, qo_indptr, num_q_heads, num_kv_heads, head_dim, v_head_dim=None, window=0,
                          sm_scale=None, sinks=None):
     v_head_dim = head_dim if v_head_dim is None else v_head_dim

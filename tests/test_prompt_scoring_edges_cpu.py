@@ -4,6 +4,7 @@ import math
 import pytest
 import torch
 
+from sglang_neuron_b200.ops.logprobs import head_logprobs, token_logprobs
 from sglang_neuron_b200.ops.prompt import prompt_attention
 
 
@@ -34,3 +35,13 @@ def test_prompt_attention_masked_places_hold_anything(bad, where, window):
     assert torch.equal(out[~hit], clean[~hit])
     if where == "v":
         assert torch.equal(out[hit], torch.full_like(out[hit], bad)) or bool(torch.isnan(out[hit]).all())
+
+
+def test_operators_are_forward_only():
+    """The CUDA kernels have no backward pass, so the PyTorch forms carry no gradient either."""
+    q = torch.randn(4, 8, requires_grad=True)
+    ip = torch.tensor([0, 4], dtype=torch.int32)
+    w, ids = torch.randn(9, 8, requires_grad=True), torch.zeros(4, dtype=torch.long)
+    outs = [prompt_attention(q, q, q, ip, 2, 2, 4), prompt_attention(q, q, q, ip, 2, 2, 4, out=torch.zeros(4, 8))]
+    outs += list(head_logprobs(q, w, ids)[:3]) + list(token_logprobs(q, ids, top_k=2)[:4])
+    assert not any(t.requires_grad for t in outs)
