@@ -457,7 +457,9 @@ __global__ void __launch_bounds__(THREADS)
 }
 
 // Joins a row's partial results. ROWS rows per CTA of 256 threads: 8 where the rows are many (their partial results
-// lie side by side), 1 where a row has many partial results and there are few rows.
+// lie side by side), 1 where a row has many partial results and there are few rows. Whole calls with 1 / 8 rows per
+// CTA, 512 x 151936: 16 rows 42.1 / 72.2 us, 128 62.1 / 97.1, 256 50.1 / 50.6, 512 85.7 / 85.5, 1024 155 / 152, 4096
+// 545 / 530; 512 x 32768: 512 24.8 / 23.8, 2048 72.6 / 65.9.
 // Tried and slower: CTAs so small that they wait beside the product's for its end (33 x 2048 x 102400: 90.7 us against
 // 85.1).
 template <int ROWS>
@@ -523,8 +525,7 @@ __global__ void __launch_bounds__(256)
 void join_parts(const at::Tensor& part, const float* chosen, int pitch, int N, int V, int tiles, int width,
                 const int64_t* ids, int64_t vocab_offset, at::Tensor& stats, cudaStream_t st) {
   float* out = stats.data_ptr<float>();
-  // one row per CTA until the CTAs would come in many waves
-  const bool one = N <= 2048;
+  const bool one = N <= 512;
   C10_CUDA_CHECK(snb::launch_pdl(one ? head_join_kernel<1> : head_join_kernel<8>, dim3(one ? N : (N + 7) / 8),
                                  dim3(256), 0, st, reinterpret_cast<const float4*>(part.data_ptr<float>()), chosen,
                                  pitch, N, V, tiles, width, ids, vocab_offset, out, out + N, out + 2 * N));
@@ -563,7 +564,9 @@ int resident_pairs(int device) {
 }
 
 // Vocabulary entries per tile. The pairs finish a round of units together, so a tile's width should make the last
-// round a full one; a narrow tile on the other hand reads hidden more often (the 32 entries added to its cost).
+// round a full one; a narrow tile on the other hand reads hidden more often (the 32 entries added to its cost). With
+// hidden rows of 2880, in us for the 32 entries / none added / always 256 wide: 300 x 32768 71 / 70 / 75, 300 x 151936
+// 333 / 366 / 326, 1000 x 102400 449 / 475 / 439, 1000 x 151936 658 / 697 / 675, 3000 x 151936 1878 / 2430 / 1874.
 int pick_width(int mt, int64_t V, int pairs) {
   int best = BN;
   int64_t least = INT64_MAX;
