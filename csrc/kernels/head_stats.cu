@@ -3,10 +3,13 @@
 //   y = z - c,  s = sum_v e^y,  t = sum_v e^y y    lse = c + log s   entropy = log s - t / s
 // A product kernel writes (c, s, t) of every vocabulary tile and row, head_join_kernel joins them.
 //
-// More than 128 rows: head_stats_kernel, bound by the tensor cores (under load by the GPU's power): 4096 x 4096 x
-// 151936 took 3123 us, 1632 TFLOP/s, where the library's product alone, in the same run, took 3219 us; 1000 x 2880 x
-// 201088 took 783 us (787 us). Up to 128 rows: head_few_kernel, bound by the weights' stream: 16 x 4096 x 151936 took
-// 219 us, 5.7 TB/s (the library's product: 211 us); at 129 rows the pair kernel takes 231 us, at 128 this one 228 us.
+// More than 128 rows: head_stats_kernel, bound by the tensor cores and, from some 0.1 s of load on, by the GPU's power:
+// 4096 x 4096 x 151936 took 3100 us, 1645 TFLOP/s, in six launches after a pause, and 3409 to 3481 us, 1465 to 1496
+// TFLOP/s, after 0.3 s of load, where the library's product alone, in the same run, took 3473 to 3491 us; 1000 x 2880 x
+// 201088 took 779 us and 884 us (883 us). Up to 128 rows: head_few_kernel, bound by the weights' stream: 16 x 4096 x
+// 151936 took 219 us, 5.7 TB/s (the library's product: 211 us); at 129 rows the pair kernel takes 258 us, at 128 this one
+// 243 us. A tiled weight arrives 16 (pair) or 32 (few) rows a load: 5495 us, 1321 us and, 33 x 2048 x 102400, 112 us
+// against 88 us row-major.
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <ATen/cuda/CUDAContext.h>

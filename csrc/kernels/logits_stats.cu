@@ -21,9 +21,9 @@
 // -2^25 and keeps 0 * y finite where a logit is masked; a CTA whose maximum is outside +-2^25 (LOWEST, HIGHEST) reads
 // its part once more on a path that subtracts first.
 // The row comes through a ring of three 16 KB bulk copies that one thread keeps full.
-// Measured on a B200: 4096 x 151936 bf16 without alternatives 234 us (5.3 TB/s), with five 254 us, with twenty 301 us
+// Measured on a B200: 4096 x 151936 bf16 without alternatives 242 us (5.1 TB/s), with five 258 us, with twenty 301 us
 // (choosing them takes a CTA some 5 us after its row); 1000 x 201088 fp32 with five 135 us (6.0 TB/s); 64 x 201088 fp32
-// without alternatives 14.2 us, with twenty 20.5 to 21.8 us. Tried and slower: CTAs that stay and load the next row's
+// without alternatives 14.3 us, with twenty 20.5 to 21.1 us. Tried and slower: CTAs that stay and load the next row's
 // first stages while they choose (280 us with five); the bound from 64 groups.
 // Split: one CTA per row, four resident per SM; fewer rows than that put a cluster of 2 to 8 CTAs on each row, whose
 // partial results the first CTA joins through distributed shared memory.

@@ -10,9 +10,13 @@
 //
 // What bounds it: the softmax warps. A block of both tiles is 2048 cycles of tensor core at head width 128 and takes
 // about 2600; per score they spend 0.75 exponentials of the special-function unit's 1/4 a cycle and scheduler (the rest
-// runs on the FMA pipe), the packing to 16 bits and the sums. Measured on a B200 (device time): one 8192-token prompt,
-// 32 / 8 heads of 128: 427 us, 1287 TFLOP/s; 64 / 8 heads of 64: 646 us, 850 TFLOP/s (the same scores at half the
-// products); 16 heads of 192 / 128: 333 us, 1031 TFLOP/s; 4096 tokens, 64 / 8 heads of 64, window 128: 44 us.
+// runs on the FMA pipe), the packing to 16 bits and the sums. Measured on a B200, 30 launches after a pause: one
+// 8192-token prompt, 32 / 8 heads of 128: 427 to 431 us, 1280 TFLOP/s (under a second's load, where power lowers the
+// clock, 498 us, 1105 TFLOP/s); 64 / 8 heads of 64: 642 us, 857 TFLOP/s (the same scores at half the products); 16 heads
+// of 192 / 128: 336 us, 1023 TFLOP/s; 4096 tokens, 64 / 8 heads of 64, window 128: 43.3 us.
+// Registers: 18 warps leave a thread 96. In bytes of stores and loads, 192 / 128 spills 56 / 84 (fp16 44 / 68), bf16 of
+// 128 / 128 8 / 12, bf16 of 64 / 64 8 / 4, the others nothing.
+// The running maximum and sum are the online softmax (Milakov and Gimelshein 2018).
 // Tried and slower: one thread per row (its chain of loads, maximum, exponentials is twice as long: 575 us); turns of
 // the two tiles at the exponentials (with one thread per row 4 % faster, with two a loss); heads of 64 with one tile
 // per CTA and two CTAs per SM (687 us against 650).
@@ -28,8 +32,9 @@
 
 namespace {
 
-// One pair of exponentials in this many runs on the FMA pipe. Cycles per block of both tiles at head width 128 with
-// one pair in 2, 3, 4, 8 and none: 2560, 2530, 2600, 2700, 3300.
+// Of each 8 pairs of exponentials those with the last index of every EMULATE run on the FMA pipe. One 8192-token prompt
+// with 4, 2 (EMULATE 3 and 4), 1 and none of 8 there: 32 / 8 heads of 128 465, 431, 421, 419 us; 64 / 8 heads of 64 742,
+// 642, 633, 685 us; 16 heads of 192 / 128 339, 336, 338, 336 us.
 constexpr int EMULATE = 4;
 constexpr float LOG2E = 1.4426950408889634f;
 

@@ -169,7 +169,8 @@ class Engine:
         come from logits in fp32, with and without alternatives.
 
         Prompts (token-id lists or strings) run whole, packed up to max_prefill_tokens tokens a forward, without
-        touching the KV cache or the scheduler. Per prompt: `input_token_logprobs` [[log-probability, id], ...]
+        touching the KV cache or the scheduler; a longer prompt is one forward, with the activations of all its tokens.
+        Per prompt: `input_token_logprobs` [[log-probability, id], ...]
         (None for the first token, which nothing precedes), `input_entropies` and `input_top_logprobs` (also None
         first). Under tensor parallelism every rank makes the same call."""
         from .ops.logprobs import MAX_TOP

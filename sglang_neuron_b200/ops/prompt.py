@@ -39,7 +39,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, qo_indpt
     """Tokens [qo_indptr[b], qo_indptr[b + 1]) are prompt b; every token attends to itself and the tokens before it
     in its prompt (the last `window` of them where window > 0). q [T, num_q_heads * head_dim], k and v [T,
     num_kv_heads * width]: bf16 or fp16 and widths of 64, 128 or 192 (values 128) on CUDA; views with a row stride
-    (columns of a fused projection) are read in place.
+    (columns of a fused projection) are read in place, rows off 16-byte boundaries are copied first.
     Returns [T, num_q_heads * v_head_dim]; rows outside every prompt are left as they are."""
     v_head_dim = head_dim if v_head_dim is None else v_head_dim
     sm_scale = head_dim ** -0.5 if sm_scale is None else sm_scale
