@@ -759,7 +759,8 @@ __global__ void __launch_bounds__(THREADS, 1)
             break;
           }
           const float most = exchange(block, [](float a, float b) { return fmaxf(a, b); });
-          const float up = most > 65536.f ? (float)((__float_as_int(most) >> 23) - 126) : 0.f;
+          // 2^-126 is the least factor that is not flushed to 0
+          const float up = most > 65536.f ? (float)min((__float_as_int(most) >> 23) - 126, 126) : 0.f;
           const float f = ex2(-up);
           l *= f;
           m += up;

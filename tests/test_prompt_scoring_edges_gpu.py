@@ -97,6 +97,30 @@ def test_prompt_attention_seen_scores_of_minus_infinity_weigh_nothing():
     assert ((out.double() - want).abs() <= (2 * U[q.dtype] + 4e-4) * A + 1e-6).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("layout", [(2, 1, 64, 64), (1, 1, 128, 128), (2, 2, 192, 128)])
+def test_prompt_attention_one_key_far_above_the_blocks_before_and_after(dtype, layout):
+    """A key whose weight is up to 2^300 of the first block's, at every step around fp32's range, with lesser keys in
+    the blocks behind it."""
+    from sglang_neuron_b200.ops.prompt import prompt_attention
+    Hq, Hkv, D, Dv = layout
+    n = 420
+    _, _, v = _qkv(n, Hq, Hkv, D, Dv, dtype, seed=41)
+    q = torch.zeros(n, Hq * D, device=DEV, dtype=dtype)
+    q.view(n, Hq, D)[..., :2] = 1.0
+    jumps = [8.0, 17.0, 100.0, 300.0] + [120.0 + 0.25 * i for i in range(44)]
+    for jump in jumps:
+        t = torch.zeros(n, device=DEV, dtype=torch.float64)
+        t[200], t[300] = jump, jump - 60.0
+        t *= math.log(2.0) * math.sqrt(D)
+        k = torch.zeros(n, Hkv, D, device=DEV, dtype=dtype)
+        k[..., 0] = t.to(dtype)[:, None]
+        k[..., 1] = (t - t.to(dtype).double()).to(dtype)[:, None]
+        k = k.view(n, Hkv * D)
+        out = prompt_attention(q, k, v, _indptr([n]), Hq, Hkv, D, v_head_dim=Dv)
+        _check_attention(out, q, k, v, [n], Hq, Hkv, D, Dv)
+
+
 def _odd_views(x):
     """The values of x in forms that tensor maps do not take as they are."""
     n, w = x.shape
